@@ -19,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "fasterllama_amd")
@@ -34,10 +35,13 @@ HIP_FLAGS = [
 ]
 
 
+HIP_SOURCES = ("fl_decode_attn.hip", "fl_kv8.hip")  # of libfl_decode_attn.so
+
+
 def sources(name: str) -> list[str]:
     """Files a target is built from (a change in any of them makes the built file stale)."""
     import glob
-    hip = [os.path.join(CSRC, "fl_decode_attn.hip")] + sorted(glob.glob(os.path.join(CSRC, "*.hpp"))) + \
+    hip = [os.path.join(CSRC, f) for f in HIP_SOURCES] + sorted(glob.glob(os.path.join(CSRC, "*.hpp"))) + \
         [os.path.join(ROOT, "include", "fl_decode_attn.h")]
     return {
         "hip": hip,
@@ -117,7 +121,12 @@ def hipcc() -> str:
 def build_hip() -> str:
     os.makedirs(LIB, exist_ok=True)
     out = os.path.join(LIB, "libfl_decode_attn.so")
-    _run([hipcc(), *HIP_FLAGS, "-shared", "-o", out, os.path.join(CSRC, "fl_decode_attn.hip")])
+    objects = [os.path.join(LIB, f.replace(".hip", ".o")) for f in HIP_SOURCES]
+    with ThreadPoolExecutor() as pool:  # a compiler process each
+        list(pool.map(lambda so: _run([hipcc(), *HIP_FLAGS, "-c", "-o", so[1], os.path.join(CSRC, so[0])]), zip(HIP_SOURCES, objects)))
+    _run([hipcc(), f"--offload-arch={GFX_ARCH}", "-shared", "-o", out, *objects])
+    for path in objects:
+        os.remove(path)
     return _built("hip")
 
 
@@ -184,7 +193,7 @@ def run_sanitizers() -> None:
           "-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
           "-Xarch_host", "-fno-sanitize-recover=all",
           "-I", os.path.join(ROOT, "include"), "-o", exe,
-          os.path.join(CSRC, "fl_decode_attn.hip"), os.path.join(ROOT, "tests", "cpp", "capi_host_check.cpp")])
+          *(os.path.join(CSRC, f) for f in HIP_SOURCES), os.path.join(ROOT, "tests", "cpp", "capi_host_check.cpp")])
     _run([exe])
 
 

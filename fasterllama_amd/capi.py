@@ -44,6 +44,13 @@ EXPORTED_SYMBOLS = (
     "fl_prefill_attn_forward_passes",
     "fl_prefill_mask_classes_bytes",
     "fl_prefill_mask_classify",
+    "fl_kv8_workspace_bytes",
+    "fl_kv8_workspace_init",
+    "fl_kv8_decode_forward",
+    "fl_kv8_prefill_forward",
+    "fl_kv8_read",
+    "fl_kv8_evict",
+    "fl_kv8_cache_bytes",
     "fl_rope_table",
     "fl_kv_cache_bytes",
     "fl_attn_strerror",
@@ -112,6 +119,44 @@ class AttnPlan(C.Structure):
     ]
 
 
+class Kv8CacheArrays(C.Structure):
+    """fl_kv8_cache; struct_size is filled in."""
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("block_len", C.c_int32),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+        ("k_tail", C.c_void_p),
+        ("v_tail", C.c_void_p),
+        ("weights", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(Kv8CacheArrays)
+
+
+class Kv8EvictArgs(C.Structure):
+    """fl_kv8_evict_args; struct_size is filled in."""
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("rows", C.c_int32),
+        ("rows_per_seq", C.c_void_p),
+        ("keep_blocks", C.c_int32),
+        ("recent_blocks", C.c_int32),
+        ("to_total_len", C.c_int32),
+        ("reserved", C.c_int32),
+        ("kept", C.c_void_p),
+        ("rows_out", C.c_void_p),
+    ]
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = C.sizeof(Kv8EvictArgs)
+
+
 class FlAttnError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"fl_decode_attn status {status}: {message}")
@@ -155,6 +200,17 @@ def load() -> C.CDLL:
     lib.fl_prefill_mask_classes_bytes.restype = C.c_int
     lib.fl_prefill_mask_classify.argtypes = [C.POINTER(AttnDesc), C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p]
     lib.fl_prefill_mask_classify.restype = C.c_int
+    desc_p, cache_p, io_p = C.POINTER(AttnDesc), C.POINTER(Kv8CacheArrays), C.POINTER(AttnIO)
+    size_p = C.POINTER(C.c_size_t)
+    lib.fl_kv8_workspace_bytes.argtypes = [desc_p, C.c_int32, C.c_int32, size_p]
+    lib.fl_kv8_workspace_init.argtypes = [desc_p, C.c_int32, C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.fl_kv8_decode_forward.argtypes = [desc_p, cache_p, io_p, C.c_void_p, C.c_void_p]
+    lib.fl_kv8_prefill_forward.argtypes = [desc_p, cache_p, io_p, C.c_int32, C.c_int32, C.c_void_p]
+    lib.fl_kv8_read.argtypes = [desc_p, cache_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.fl_kv8_evict.argtypes = [desc_p, cache_p, cache_p, C.POINTER(Kv8EvictArgs), C.c_void_p]
+    lib.fl_kv8_cache_bytes.argtypes = [desc_p, C.c_int32, size_p, size_p, size_p]
+    for name in ("workspace_bytes", "workspace_init", "decode_forward", "prefill_forward", "read", "evict", "cache_bytes"):
+        getattr(lib, "fl_kv8_" + name).restype = C.c_int
     lib.fl_rope_table.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_float, C.c_void_p]
     lib.fl_rope_table.restype = C.c_int
     lib.fl_attn_strerror.argtypes = [C.c_int]

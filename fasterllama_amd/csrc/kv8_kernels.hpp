@@ -1,0 +1,1002 @@
+// Kernels of the 8-bit key/value cache for gfx950: decode step, prompt-phase append, read-back, eviction.
+//
+// The cache of one layer holds K and V rows as signed bytes [B,H,L,D] with one float scale per block of T rows and head
+// [B,H,L/T].  The rows of the block that is not full yet wait in fp16 in a tail [B,H,T,D]; the step that brings the last row
+// of a block quantises all T of them at once, so a row is rounded to 8 bits exactly once, whatever mix of prompt pieces and
+// decode steps filled its block.
+//   stored row     x -> fp16, nearest-even; a non-finite value becomes 0 and a finite one stays within +-65504, so that one
+//                  bad element (padding, say) can neither turn the scale of its T rows into NaN nor into infinity
+//   block          scale = absmax / 127, integer = rint(x * (127 / absmax)), all in FP32; absmax = 0: zeros
+// Attention reads the cache as it stands after the append: integers * scale for complete blocks, the fp16 tail behind them.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "decode_attn_kernels.hpp"
+#include "prefill_attn_kernels.hpp"
+
+#pragma clang fp contract(off)
+
+namespace flattn {
+
+enum { kInF32 = 0, kInF16 = 1, kInI32 = 2 }; // what q / k_new / v_new hold
+
+struct Kv8Params {
+    Params a;      // inputs, mask, positions, partials (k_cache / v_cache unused); B, H, L, scale, plan
+    int8_t *k8, *v8;          // [B*H, L, D]
+    float *k_scale, *v_scale; // [B*H, nblk]
+    _Float16 *k_tail, *v_tail; // [B*H, T, D]
+    float *weights;           // [B*H, nblk] accumulated softmax weight, or NULL
+    float2 *granules;         // workspace [B*H, L / granule rows]: (reference maximum, sum of weights) of a few rows
+    const int32_t *rope_rows; // [B] table rows, or NULL: a.rope_row
+    int32_t in_kind;
+    int32_t T, t_shift;       // rows per block, log2
+    int32_t nblk;             // L / T
+    int32_t S;                // queries per sequence (prompt phase)
+    float2 *stats;            // prompt phase, workspace [B*H, S]: (maximum, sum) of every query's softmax, or NULL
+    int32_t weight_queries;   // the last of them whose weights are gathered
+};
+
+// ---------------------------------------------------------------- inputs and stored values
+
+// N consecutive elements of an input tensor as float.  The input format is uniform: one straight run of loads each.
+template <int N>
+__device__ __forceinline__ void load_input(const void *base, int kind, size_t off, float inp_scale, const float *w_scale_at, float (&dst)[N])
+{
+    if (kind == kInF16) {
+        half8 v[N / 8];
+#pragma unroll
+        for (int i = 0; i < N / 8; ++i) v[i] = reinterpret_cast<const half8 *>(reinterpret_cast<const _Float16 *>(base) + off)[i];
+#pragma unroll
+        for (int i = 0; i < N; ++i) dst[i] = (float)v[i / 8][i % 8];
+    } else if (kind == kInF32) {
+        float4 v[N / 4];
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) v[i] = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(base) + off)[i];
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) { dst[4 * i] = v[i].x; dst[4 * i + 1] = v[i].y; dst[4 * i + 2] = v[i].z; dst[4 * i + 3] = v[i].w; }
+    } else { // (float)acc * inp_scale * w_scale, left to right, as the other caches' kernels
+        int4 v[N / 4];
+        float4 w[N / 4];
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            v[i] = reinterpret_cast<const int4 *>(reinterpret_cast<const int32_t *>(base) + off)[i];
+            w[i] = reinterpret_cast<const float4 *>(w_scale_at)[i];
+        }
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            dst[4 * i + 0] = __fmul_rn(__fmul_rn((float)v[i].x, inp_scale), w[i].x);
+            dst[4 * i + 1] = __fmul_rn(__fmul_rn((float)v[i].y, inp_scale), w[i].y);
+            dst[4 * i + 2] = __fmul_rn(__fmul_rn((float)v[i].z, inp_scale), w[i].z);
+            dst[4 * i + 3] = __fmul_rn(__fmul_rn((float)v[i].w, inp_scale), w[i].w);
+        }
+    }
+}
+
+// RoPE of N consecutive elements by their table entries.
+template <int N>
+__device__ __forceinline__ void rotate_run(float (&x)[N], const float *freq_at)
+{
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 f = *reinterpret_cast<const float4 *>(freq_at + i);
+        float r0, r1, r2, r3;
+        rope_pair(x[i], x[i + 1], f.x, f.y, r0, r1);
+        rope_pair(x[i + 2], x[i + 3], f.z, f.w, r2, r3);
+        x[i] = r0; x[i + 1] = r1; x[i + 2] = r2; x[i + 3] = r3;
+    }
+}
+
+__device__ __forceinline__ _Float16 stored_half(float x)
+{
+    const float y = fminf(fmaxf(x, -65504.f), 65504.f);
+    return to_storage<_Float16>(__builtin_isfinite(x) ? y : 0.f);
+}
+
+// 127 / absmax; 0 for a block of zeros
+__device__ __forceinline__ float quant_factor(float absmax) { return absmax > 0.f ? 127.0f / absmax : 0.f; }
+// |x * factor| < 127.5 by construction: no clamp
+__device__ __forceinline__ int quantise(float x, float factor) { return (int)rintf(__fmul_rn(x, factor)); }
+
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d)
+{
+    return ((uint32_t)a & 0xffu) | ((uint32_t)b & 0xffu) << 8 | ((uint32_t)c & 0xffu) << 16 | (uint32_t)d << 24;
+}
+
+template <int I>
+__device__ __forceinline__ float byte_float(uint32_t x) { return (float)(int8_t)(x >> (8 * I)); }
+
+// ---------------------------------------------------------------- reductions across the rows of a wave
+
+__device__ __forceinline__ float swap16(float x, float &other) // other: the value of lane ^ 16 (in one of the two orders)
+{
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    other = __uint_as_float(r[1]);
+    return __uint_as_float(r[0]);
+}
+__device__ __forceinline__ float swap32(float x, float &other)
+{
+    const unsigned u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    other = __uint_as_float(r[1]);
+    return __uint_as_float(r[0]);
+}
+
+// Maximum / sum over the 64 / LPR lane groups of a wave; within a group of LPR lanes the input is the same (cross_max) or a
+// value of its own per lane (cross_sum, which adds equal lanes of the groups).
+template <int LPR>
+__device__ __forceinline__ float cross_max(float x)
+{
+    float y;
+    if constexpr (LPR <= 1) x = fmaxf(x, dpp_move<0xB1>(x));
+    if constexpr (LPR <= 2) x = fmaxf(x, dpp_move<0x4E>(x));  // lane ^ 2
+    if constexpr (LPR <= 4) x = fmaxf(x, dpp_move<0x141>(x)); // the other four of eight
+    if constexpr (LPR <= 8) x = fmaxf(x, dpp_move<0x140>(x)); // the other eight of sixteen
+    if constexpr (LPR <= 16) { x = swap16(x, y); x = fmaxf(x, y); }
+    if constexpr (LPR <= 32) { x = swap32(x, y); x = fmaxf(x, y); }
+    return x;
+}
+template <int LPR>
+__device__ __forceinline__ float cross_sum(float x)
+{
+    float y;
+    static_assert(LPR >= 2, "a row has at least two 16-byte chunks");
+    if constexpr (LPR <= 2) x += dpp_move<0x4E>(x);                 // lane ^ 2
+    if constexpr (LPR <= 4) x += __shfl_xor(x, 4);                  // (a mirror would pair unequal lanes of the groups)
+    if constexpr (LPR <= 8) x += dpp_move<0x128>(x);                // row_ror:8 = lane ^ 8
+    if constexpr (LPR <= 16) { x = swap16(x, y); x += y; }
+    if constexpr (LPR <= 32) { x = swap32(x, y); x += y; }
+    return x;
+}
+
+// ---------------------------------------------------------------- decode step
+
+template <int D>
+struct Kv8Geometry {
+    static constexpr int CH = D / 16;               // 16-byte chunks per row: one per lane
+    static constexpr int LPR = lanes_per_row(CH);   // lanes per row
+    static constexpr bool PADDED = LPR != CH;       // size_per_head 96: two of eight lanes own no chunk
+    static constexpr int GPW = 64 / LPR;            // rows per wave and load instruction; at most 32, so inside one block
+    static constexpr int U = 4;                     // load instructions per matrix in flight
+    static constexpr int WT = GPW * U;              // rows per wave and trip
+    static constexpr int GR = WT < 32 ? WT : 32;    // rows per granule of the weight sums
+    static constexpr int NS = WT > 32 ? WT / 32 : 1; // 32-row groups per trip: each has one scale
+};
+
+constexpr float kKv8LazyMax = 8.0f; // base-2 units: the running reference maximum may lag the true one by this much
+constexpr float kQDigits = 8300000.0f; // |q| maps to at most this: three balanced base-256 digits reach 8355711
+constexpr int kKv8Waves = 4;
+
+// Adds the softmax weight of every block to weights[b,h,:], from the granules and the merged statistics (M, Lsum) of the
+// row.  A block whose first row arrived in this step starts from 0.
+template <int D>
+__device__ __forceinline__ void add_block_weights(const Kv8Params &p, int bh, int P, float M, float Lsum, int tid)
+{
+    constexpr int GR = Kv8Geometry<D>::GR;
+    if (!(Lsum > 0.f)) return; // every key masked: the output is NaN, nothing was attended to
+    const int blk_new = P >> p.t_shift;
+    const bool open = ((P + 1) & (p.T - 1)) != 0; // the last block's rows are in the tail: one granule for all of them
+    const float2 *g = p.granules + (size_t)bh * (p.a.L / GR);
+    const int per = p.T / GR;
+    const float rl = 1.0f / Lsum;
+    for (int blk = tid; blk <= blk_new; blk += kKv8Waves * 64) {
+        float w = 0.f;
+        const int n = open && blk == blk_new ? 1 : per;
+        for (int i = 0; i < n; ++i) {
+            const float *e = reinterpret_cast<const float *>(g + (size_t)blk * per + i);
+            const float m = load_partial<true>(e), s = load_partial<true>(e + 1);
+            w = fmaf(s, __builtin_amdgcn_exp2f(m - M), w);
+        }
+        float *dst = p.weights + (size_t)bh * p.nblk + blk;
+        const bool fresh = blk == blk_new && (P & (p.T - 1)) == 0;
+        *dst = fresh ? w * rl : fmaf(w, rl, *dst);
+    }
+}
+
+// Quantises one full tail (T rows of one (b,h)) into block `blk`, by the 256 threads of a workgroup.  Two passes over
+// the tail: T * D halfs, which the second finds in the caches.
+template <int D>
+__device__ __forceinline__ void quantise_tail(const _Float16 *tail, int8_t *rows8, float *scale_at, int T, float *s_red)
+{
+    const int tid = threadIdx.x, n8 = T * (D / 8);
+    const half8 *src = reinterpret_cast<const half8 *>(tail);
+    float absmax = 0.f;
+    for (int i = tid; i < n8; i += kKv8Waves * 64) {
+        const half8 x = src[i];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) absmax = fmaxf(absmax, fabsf((float)x[j]));
+    }
+    absmax = wave_max(absmax);
+    __syncthreads(); // s_red is free
+    if ((tid & 63) == 0) s_red[tid >> 6] = absmax;
+    __syncthreads();
+    absmax = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    const float f = quant_factor(absmax);
+    for (int i = tid; i < n8; i += kKv8Waves * 64) {
+        const half8 x = src[i];
+        uint2 o;
+        o.x = pack4(quantise((float)x[0], f), quantise((float)x[1], f), quantise((float)x[2], f), quantise((float)x[3], f));
+        o.y = pack4(quantise((float)x[4], f), quantise((float)x[5], f), quantise((float)x[6], f), quantise((float)x[7], f));
+        reinterpret_cast<uint2 *>(rows8)[i] = o;
+    }
+    if (tid == 0) *scale_at = absmax / 127.0f;
+}
+
+// One decode step (PROMPT = false): grid = splits * B * H workgroups of four waves, (b,h) fastest as in the streaming
+// kernel of the other cache types; a workgroup streams `chunk` rows (a multiple of 128) of one (b,h), four rows per lane
+// group and trip.  PROMPT = true: one workgroup per (b, query, h) over the rows as they are, no append — the prompt phase
+// of the head sizes the matrix-core kernel does not serve.
+//
+// A row of D bytes is D/16 lanes.  Scores: the query enters as integers of three base-256 digits, q = qs * (d0 + 256 d1 +
+// 65536 d2) with |error| <= 2^-24 of its largest element, so K needs no conversion: twelve v_dot4_i32_i8 per 16 bytes
+// multiply the bytes as they come (exactly), against 32 instructions for conversion and FMA.  V bytes are converted (one
+// instruction each) and accumulated in FP32.  The running maximum is shared by the whole wave, which makes the weights of
+// different rows comparable at once (granule sums) and the rescale of the accumulators a rare, wave-uniform branch.
+template <int D, bool HAS_MASK, bool PROMPT>
+__global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Params p)
+{
+    typedef Kv8Geometry<D> G;
+    constexpr int LPR = G::LPR, GPW = G::GPW, U = G::U, WT = G::WT, GR = G::GR;
+    static_assert(kKv8Waves * 64 == kCombineThreads, "the merge runs on a 256-thread workgroup");
+    __shared__ float s_o[kKv8Waves][D];
+    __shared__ float s_m[kKv8Waves], s_l[kKv8Waves], s_t[kKv8Waves], s_red[kKv8Waves];
+    __shared__ CombineShared<D> s_merge;
+    __shared__ int s_last;
+
+    const Params &a = p.a;
+    const int H = a.H, L = a.L, T = p.T;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane / LPR, lig = lane % LPR;
+    int split = 0, bh, b, h, P, s_query = 0;
+    if constexpr (PROMPT) { // blockIdx = (b * S + s) * H + h
+        h = blockIdx.x % H;
+        const int bs = blockIdx.x / H;
+        b = bs / p.S;
+        s_query = bs % p.S;
+        bh = b * H + h;
+        P = a.start_pos + p.S - 1; // the last row in the cache
+    } else {
+        const int BH = a.B * H;
+        split = blockIdx.x / BH;
+        bh = blockIdx.x % BH;
+        b = bh / H;
+        h = bh % H;
+        P = a.pos_per_seq ? a.pos_per_seq[b] : a.start_pos;
+        if (P < 0 || P >= L || P > a.max_pos) { // outside the cache or the plan: store nothing, poison the output
+            if ((a.direct || a.arrivals) && split == 0)
+                for (int d = tid; d < D; d += kKv8Waves * 64) a.out[(size_t)bh * D + d] = __builtin_nanf("");
+            return;
+        }
+    }
+    const int ctx = P + 1;
+    const int start = PROMPT ? 0 : split * a.chunk;
+    if (start >= ctx) return;
+    const int end = PROMPT ? ctx : min(start + a.chunk, ctx);
+    const bool owner = end == ctx;                     // this workgroup has the newest row
+    const int P0 = P & ~(T - 1);
+    const bool fills = ctx == P0 + T;                  // the newest row is the last of its block
+    const int end8 = owner && !fills ? P0 : end;       // rows [start, end8) come as bytes; multiples of T
+    const int q_pos = PROMPT ? a.start_pos + s_query : P;
+    const size_t row_off = (size_t)bh * L * D, tail_off = (size_t)bh * T * D;
+    const bool has_chunk = !G::PADDED || lig < G::CH;
+    const int e0 = lig * 16;
+
+    const float inp_scale = p.in_kind == kInI32 ? a.inp_scale[PROMPT ? b * p.S + s_query : b] : 0.f;
+    int rope_row = PROMPT ? (a.rope_row < 0 ? q_pos : a.rope_row + s_query) : (a.rope_row < 0 ? P : a.rope_row);
+    if (!PROMPT && p.rope_rows) rope_row = p.rope_rows[b];
+    const float *freq = a.freq_cis + (size_t)rope_row * D + e0;
+    const size_t in_off = PROMPT ? ((size_t)(b * p.S + s_query) * H + h) * D + e0 : (size_t)bh * D + e0;
+
+    // The append: the new row goes to the tail; where it completes the block, the workgroup quantises the tail, and
+    // the loop below finds those rows as bytes.
+    half8 kn[2], vn[2];
+    if (!PROMPT && owner) {
+        if (wave == 0 && has_chunk) {
+            float x[16], y[16];
+            load_input<16>(a.k_new, p.in_kind, in_off, inp_scale, p.in_kind == kInI32 ? a.wk_scale + h * D + e0 : nullptr, x);
+            load_input<16>(a.v_new, p.in_kind, in_off, inp_scale, p.in_kind == kInI32 ? a.wv_scale + h * D + e0 : nullptr, y);
+            rotate_run<16>(x, freq);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { kn[i / 8][i % 8] = stored_half(x[i]); vn[i / 8][i % 8] = stored_half(y[i]); }
+            if (g == 0) {
+                const size_t at = tail_off + (size_t)(P - P0) * D + e0;
+                half8 *kd = reinterpret_cast<half8 *>(p.k_tail + at), *vd = reinterpret_cast<half8 *>(p.v_tail + at);
+                kd[0] = kn[0]; kd[1] = kn[1];
+                vd[0] = vn[0]; vd[1] = vn[1];
+            }
+        }
+        if (fills) {
+            __syncthreads(); // the new row is in the tail
+            const int blk = P >> p.t_shift;
+            quantise_tail<D>(p.k_tail + tail_off, p.k8 + row_off + (size_t)P0 * D, p.k_scale + (size_t)bh * p.nblk + blk, T, s_red);
+            quantise_tail<D>(p.v_tail + tail_off, p.v8 + row_off + (size_t)P0 * D, p.v_scale + (size_t)bh * p.nblk + blk, T, s_red);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads(); // and the block in the cache
+        }
+    }
+
+    // The rotated query
+    float qf[16];
+    if (has_chunk) {
+        load_input<16>(a.q, p.in_kind, in_off, inp_scale, p.in_kind == kInI32 ? a.wq_scale + h * D + e0 : nullptr, qf);
+        rotate_run<16>(qf, freq);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) qf[i] = 0.f;
+    }
+
+    const float scale = a.scale * kLog2e;
+    const float floor_m = kMaxFloor * kLog2e;
+    const float *mrow = HAS_MASK ? a.attn_mask + (size_t)q_pos * a.mask_ld : nullptr;
+    float m = floor_m, l = 0.f, lt = 0.f; // wave-uniform maximum; this lane group's sums over all rows / the tail rows
+    float o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = 0.f;
+    auto raise = [&](float top) __attribute__((always_inline)) { // top: wave-uniform
+        if (__builtin_amdgcn_readfirstlane((int)(top > m + kKv8LazyMax))) {
+            const float alpha = __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= alpha;
+            lt *= alpha;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= alpha;
+        }
+    };
+
+    // The tail: fp16 rows [P0, P], the newest from registers.  Two rows per lane group and trip.
+    if (owner && !fills) {
+        const int n = PROMPT ? ctx - P0 : P - P0; // rows to be read
+        const _Float16 *kt = p.k_tail + tail_off + e0, *vt = p.v_tail + tail_off + e0;
+        constexpr int UT = 2;
+        for (int r0 = wave * GPW * UT; r0 < n; r0 += kKv8Waves * GPW * UT) {
+            half8 kx[UT][2], vx[UT][2];
+            float s[UT], mk[UT];
+            bool ok[UT];
+#pragma unroll
+            for (int u = 0; u < UT; ++u) {
+                const int r = r0 + u * GPW + g;
+                ok[u] = r < n;
+                const size_t at = (size_t)min(r, n - 1) * D;
+                if (has_chunk) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        kx[u][c] = reinterpret_cast<const half8 *>(kt + at)[c];
+                        vx[u][c] = reinterpret_cast<const half8 *>(vt + at)[c];
+                    }
+                } else {
+                    kx[u][0] = kx[u][1] = vx[u][0] = vx[u][1] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+                }
+                mk[u] = HAS_MASK ? mrow[P0 + min(r, n - 1)] * kLog2e : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < UT; ++u) {
+                float acc = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc = fmaf((float)kx[u][i / 8][i % 8], qf[i], acc);
+                s[u] = acc;
+            }
+            group_sum_n<LPR, UT>(s);
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int u = 0; u < UT; ++u) {
+                s[u] = ok[u] ? (HAS_MASK ? fmaf(s[u], scale, mk[u]) : s[u] * scale) : -__builtin_inff();
+                top = fmaxf(top, s[u]);
+            }
+            raise(cross_max<LPR>(top));
+#pragma unroll
+            for (int u = 0; u < UT; ++u) {
+                const float e = __builtin_amdgcn_exp2f(s[u] - m);
+                l += e;
+                lt += e;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = fmaf(e, (float)vx[u][i / 8][i % 8], o[i]);
+            }
+        }
+        if (!PROMPT && wave == 0) { // the new row: every lane group has it, group 0 counts it
+            float acc = 0.f;
+            if (has_chunk) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc = fmaf((float)kn[i / 8][i % 8], qf[i], acc);
+            }
+            acc = group_sum<LPR>(acc);
+            const float s = HAS_MASK ? fmaf(acc, scale, mrow[P] * kLog2e) : acc * scale;
+            raise(s);
+            if (g == 0) {
+                const float e = __builtin_amdgcn_exp2f(s - m);
+                l += e;
+                lt += e;
+                if (has_chunk) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = fmaf(e, (float)vn[i / 8][i % 8], o[i]);
+                }
+            }
+        }
+    }
+
+    // The query as three digits per element.  A non-finite element makes the factor NaN, as it would every score.
+    uint32_t qd[3][4];
+    float qs;
+    {
+        float top = 0.f, bad = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { top = fmaxf(top, fabsf(qf[i])); bad += qf[i] * 0.f; }
+        if constexpr (LPR >= 2) top = fmaxf(top, dpp_move<0xB1>(top));
+        if constexpr (LPR >= 4) top = fmaxf(top, dpp_move<0x4E>(top));
+        if constexpr (LPR >= 8) top = fmaxf(top, dpp_move<0x141>(top));
+        if constexpr (LPR >= 16) top = fmaxf(top, dpp_move<0x140>(top));
+        if constexpr (LPR >= 32) top = fmaxf(top, __shfl_xor(top, 16));
+        if constexpr (LPR >= 64) top = fmaxf(top, __shfl_xor(top, 32));
+        bad = group_sum<LPR>(bad);
+        top = fmaxf(top, 1e-30f);
+        const float f = kQDigits / top;
+        qs = (top / kQDigits + bad) * scale;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = (uint32_t)((int)rintf(qf[4 * j + i] * f) + 0x808080); // digits + 128, in bytes
+#pragma unroll
+            for (int d = 0; d < 3; ++d)
+                qd[d][j] = (((y[0] >> (8 * d)) & 0xffu) | ((y[1] >> (8 * d)) & 0xffu) << 8 | ((y[2] >> (8 * d)) & 0xffu) << 16 |
+                            ((y[3] >> (8 * d)) & 0xffu) << 24) ^ 0x80808080u;
+        }
+    }
+
+    // The byte rows
+    const __amdgpu_buffer_rsrc_t Kbuf = make_buffer(p.k8 + row_off), Vbuf = make_buffer(p.v8 + row_off);
+    const __amdgpu_buffer_rsrc_t Mbuf = make_buffer(HAS_MASK ? (const void *)mrow : (const void *)p.k8);
+    const float *ks_at = p.k_scale + (size_t)bh * p.nblk, *vs_at = p.v_scale + (size_t)bh * p.nblk;
+    const uint32_t lane_off = has_chunk ? (uint32_t)(g * D + e0) : kLaneOutOfRange;
+    const bool gather = !PROMPT && p.weights != nullptr;
+
+    auto trip = [&](int r, auto check_tag) __attribute__((always_inline)) {
+        constexpr bool CHECK = decltype(check_tag)::value;
+        u32x4 kv[U], vv[U];
+        float mk[U], ks[G::NS], vs[G::NS];
+        bool ok[U]; // uniform: a load instruction's rows are whole blocks' or whole parts of one
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            ok[u] = !CHECK || r + u * GPW < end8;
+            if constexpr (HAS_MASK)
+                mk[u] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(Mbuf, ok[u] ? (uint32_t)g * 4u : kLaneOutOfRange,
+                                                                                       (uint32_t)(r + u * GPW) * 4u, 0));
+        }
+#pragma unroll
+        for (int n = 0; n < G::NS; ++n) {
+            const int blk = min((r + 32 * n) >> p.t_shift, p.nblk - 1);
+            ks[n] = ks_at[blk];
+            vs[n] = !CHECK || r + 32 * n < end8 ? vs_at[blk] : 0.f; // (a block that was never written may have any scale)
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            kv[u] = __builtin_amdgcn_raw_buffer_load_b128(Kbuf, ok[u] ? lane_off : kLaneOutOfRange, (uint32_t)(r + u * GPW) * (uint32_t)D, kLoadNonTemporal);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            vv[u] = __builtin_amdgcn_raw_buffer_load_b128(Vbuf, ok[u] ? lane_off : kLaneOutOfRange, (uint32_t)(r + u * GPW) * (uint32_t)D, kLoadNonTemporal);
+        __builtin_amdgcn_sched_barrier(0);
+
+        float s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            int acc[3] = {0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int d = 0; d < 3; ++d) acc[d] = __builtin_amdgcn_sdot4((int)kv[u][j], (int)qd[d][j], acc[d], false);
+            // 16 products of at most 127 * 128: the two low digits fit one integer, the top digit's weight is 65536
+            s[u] = fmaf((float)acc[2], 65536.f, (float)(acc[0] + (acc[1] << 8)));
+        }
+        group_sum_n<LPR, U>(s);
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float f = qs * ks[u * GPW / 32];
+            s[u] = HAS_MASK ? fmaf(s[u], f, mk[u] * kLog2e) : s[u] * f;
+            if (CHECK && !ok[u]) s[u] = -__builtin_inff();
+            top = fmaxf(top, s[u]);
+        }
+        raise(cross_max<LPR>(top));
+        float e[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            e[u] = __builtin_amdgcn_exp2f(s[u] - m);
+            l += e[u];
+            const float w = e[u] * vs[u * GPW / 32];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[4 * j + 0] = fmaf(w, byte_float<0>(vv[u][j]), o[4 * j + 0]);
+                o[4 * j + 1] = fmaf(w, byte_float<1>(vv[u][j]), o[4 * j + 1]);
+                o[4 * j + 2] = fmaf(w, byte_float<2>(vv[u][j]), o[4 * j + 2]);
+                o[4 * j + 3] = fmaf(w, byte_float<3>(vv[u][j]), o[4 * j + 3]);
+            }
+        }
+        if (gather) {
+            constexpr int NG = WT / GR, UG = U / NG; // granules per trip, load instructions per granule
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                if (CHECK && !ok[n * UG]) continue; // a granule is whole or absent: T and the chunk are multiples of it
+                float sum = 0.f;
+#pragma unroll
+                for (int u = 0; u < UG; ++u) sum += e[n * UG + u];
+                sum = cross_sum<LPR>(sum);
+                float *dst = reinterpret_cast<float *>(p.granules + (size_t)bh * (L / GR) + r / GR + n);
+                if (lane == 0) {
+                    store_partial<true>(dst, m);
+                    store_partial<true>(dst + 1, sum);
+                }
+            }
+        }
+    };
+    int r = start + wave * WT;
+    for (; r + WT <= end8; r += kKv8Waves * WT) trip(r, std::false_type{});
+    if (r < end8) trip(r, std::true_type{});
+
+    // Merge: lane groups in registers, waves through LDS.
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = cross_sum<LPR>(o[i]);
+    l = cross_sum<LPR>(l);
+    lt = cross_sum<LPR>(lt);
+    if (g == 0 && has_chunk) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4 *>(&s_o[wave][e0 + i]) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+    }
+    if (lane == 0) {
+        s_m[wave] = m;
+        s_l[wave] = l;
+        s_t[wave] = lt;
+    }
+    __syncthreads();
+    float M = s_m[0];
+#pragma unroll
+    for (int w = 1; w < kKv8Waves; ++w) M = fmaxf(M, s_m[w]);
+    float f[kKv8Waves], Lsum = 0.f, Lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < kKv8Waves; ++w) {
+        f[w] = __builtin_amdgcn_exp2f(s_m[w] - M);
+        Lsum = fmaf(s_l[w], f[w], Lsum);
+        Lt = fmaf(s_t[w], f[w], Lt);
+    }
+    if (gather && owner && !fills && tid == 0) { // the open block's weight as its first granule
+        float *dst = reinterpret_cast<float *>(p.granules + (size_t)bh * (L / GR) + P0 / GR);
+        store_partial<true>(dst, M);
+        store_partial<true>(dst + 1, Lt);
+    }
+    const size_t slot = (size_t)bh * a.split_cap + split;
+    const bool direct = PROMPT || a.direct;
+    for (int d = tid; d < D; d += kKv8Waves * 64) {
+        float O = 0.f;
+#pragma unroll
+        for (int w = 0; w < kKv8Waves; ++w) O = fmaf(s_o[w][d], f[w], O);
+        if (direct) a.out[(PROMPT ? (size_t)bh * p.S + s_query : (size_t)bh) * D + d] = O / Lsum;
+        else store_partial<true>(a.part_o + slot * D + d, O);
+    }
+    if (PROMPT) {
+        if (p.stats && tid == 0) p.stats[(size_t)bh * p.S + s_query] = make_float2(M, Lsum);
+        return;
+    }
+    if (direct) {
+        if (gather) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads(); // every wave's granules are written
+            add_block_weights<D>(p, bh, P, M, Lsum, tid);
+        }
+        return;
+    }
+    if (tid == 0) {
+        store_partial<true>(a.part_m + slot, M);
+        store_partial<true>(a.part_l + slot, Lsum);
+    }
+    if (!a.arrivals) return;
+    // Publish -> count -> merge, ordered as in the streaming kernel of the other cache types: device-coherent stores, a wait
+    // for their acknowledgement in every thread, the barrier, the device-scope count, the barrier, device-coherent loads.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const int nsp = active_splits(a, P);
+    if (tid == 0) {
+        const int before = __hip_atomic_fetch_add(a.arrivals + bh, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = before == nsp - 1;
+        if (before == nsp - 1) __hip_atomic_store(a.arrivals + bh, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (s_last) {
+        const float2 ml = combine_partials<D, true>(a, bh, nsp, tid, s_merge);
+        if (gather) add_block_weights<D>(p, bh, P, ml.x, ml.y, tid);
+    }
+}
+
+// grid = B*H, block = 256: the merge as a launch of its own.
+template <int D>
+__global__ __launch_bounds__(kCombineThreads) void kv8_combine_kernel(const Kv8Params p)
+{
+    __shared__ CombineShared<D> sh;
+    const int bh = blockIdx.x, tid = threadIdx.x, b = bh / p.a.H;
+    const int P = p.a.pos_per_seq ? p.a.pos_per_seq[b] : p.a.start_pos;
+    if (P < 0 || P >= p.a.L || P > p.a.max_pos) {
+        for (int d = tid; d < D; d += kCombineThreads) p.a.out[(size_t)bh * D + d] = __builtin_nanf("");
+        return;
+    }
+    const float2 ml = combine_partials<D, false>(p.a, bh, active_splits(p.a, P), tid, sh);
+    if (p.weights) add_block_weights<D>(p, bh, P, ml.x, ml.y, tid);
+}
+
+// ---------------------------------------------------------------- prompt phase: append
+
+// grid = max(complete blocks, 1) * 2 * B*H: one workgroup per block of rows that the call completes, K and V apart, heads
+// fastest (neighbours read neighbouring heads of the same tokens); block = 256.  The first workgroup of a (b,h) is the one that reads the tail (its block may begin with rows of an
+// earlier call), and therefore also the one that stores the rows of the last, incomplete block there, behind a barrier.
+// Bound by the traffic: inputs once, a byte per value out.
+template <int D, int T>
+__global__ __launch_bounds__(256) void kv8_append_kernel(const Kv8Params p)
+{
+    constexpr int CPR = D / 8;                        // 8-element chunks per row
+    constexpr int NI = (T * CPR + 255) / 256;         // chunks per thread
+    constexpr bool EXACT = (T * CPR) % 256 == 0;
+    constexpr bool KEEP = NI <= 16;                   // the rounded rows stay in registers between the two passes
+    __shared__ float s_red[4];
+    const Params &a = p.a;
+    const int BH = a.B * a.H;
+    const int tid = threadIdx.x, bh = blockIdx.x % BH, b = bh / a.H, h = bh % a.H;
+    const bool is_v = (blockIdx.x / BH & 1) != 0;
+    const int nth = blockIdx.x / BH >> 1; // of the blocks this call touches
+    const int P = a.start_pos, end = P + p.S;
+    const int first = P / T, last = end / T;          // blocks [first, last) are complete after the call
+    _Float16 *tail = (is_v ? p.v_tail : p.k_tail) + (size_t)bh * T * D;
+    const void *src = is_v ? a.v_new : a.k_new;
+    const float *w = is_v ? a.wv_scale : a.wk_scale;
+
+    auto new_chunk = [&](int row, int e0) __attribute__((always_inline)) -> half8 { // row of the cache, P <= row < end
+        const int64_t token = (int64_t)b * p.S + (row - P);
+        const float inp_scale = p.in_kind == kInI32 ? a.inp_scale[token] : 0.f;
+        float x[8];
+        load_input<8>(src, p.in_kind, (size_t)(token * a.H + h) * D + e0, inp_scale, p.in_kind == kInI32 ? w + h * D + e0 : nullptr, x);
+        if (!is_v) rotate_run<8>(x, a.freq_cis + (size_t)(a.rope_row < 0 ? row : a.rope_row + (row - P)) * D + e0);
+        half8 y;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = stored_half(x[i]);
+        return y;
+    };
+    const int blk = first + nth;
+    if (blk < last) {
+        auto chunk = [&](int i) __attribute__((always_inline)) -> half8 { // chunk i of the block's T * CPR
+            const int row = blk * T + i / CPR, e0 = (i % CPR) * 8;
+            if (row < P) return *reinterpret_cast<const half8 *>(tail + (size_t)(i / CPR) * D + e0);
+            return new_chunk(row, e0);
+        };
+        half8 kept[KEEP ? NI : 1];
+        float absmax = 0.f;
+#pragma unroll KEEP ? NI : 1
+        for (int n = 0; n < NI; ++n) {
+            const int i = tid + n * 256;
+            half8 x = half8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (EXACT || i < T * CPR) x = chunk(i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) absmax = fmaxf(absmax, fabsf((float)x[j]));
+            if constexpr (KEEP) kept[n] = x;
+        }
+        absmax = wave_max(absmax);
+        if ((tid & 63) == 0) s_red[tid >> 6] = absmax;
+        __syncthreads();
+        absmax = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+        const float f = quant_factor(absmax);
+        uint2 *dst = reinterpret_cast<uint2 *>((is_v ? p.v8 : p.k8) + ((size_t)bh * a.L + (size_t)blk * T) * D);
+#pragma unroll KEEP ? NI : 1
+        for (int n = 0; n < NI; ++n) {
+            const int i = tid + n * 256;
+            if (!EXACT && i >= T * CPR) continue;
+            const half8 x = KEEP ? kept[KEEP ? n : 0] : chunk(i);
+            uint2 o;
+            o.x = pack4(quantise((float)x[0], f), quantise((float)x[1], f), quantise((float)x[2], f), quantise((float)x[3], f));
+            o.y = pack4(quantise((float)x[4], f), quantise((float)x[5], f), quantise((float)x[6], f), quantise((float)x[7], f));
+            dst[i] = o;
+        }
+        if (tid == 0) (is_v ? p.v_scale : p.k_scale)[(size_t)bh * p.nblk + blk] = absmax / 127.0f;
+    }
+    if (nth == 0) {
+        __syncthreads(); // the tail's old rows have been read
+        const int r0 = max(last * T, P);
+        for (int i = tid; i < (end - r0) * CPR; i += 256) {
+            const int row = r0 + i / CPR, e0 = (i % CPR) * 8;
+            *reinterpret_cast<half8 *>(tail + (size_t)(row - last * T) * D + e0) = new_chunk(row, e0);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- prompt phase: block weights
+
+// weights[b,h,blk] (+)= sum over the last weight_queries queries and the block's rows of e^(s - M) / sum, with the statistics
+// the attention kernel left.  grid = blocks * B*H, block = 256; a lane group owns up to four rows of the block.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_prompt_weights_kernel(const Kv8Params p)
+{
+    typedef Kv8Geometry<D> G;
+    constexpr int LPR = G::LPR, R = 4; // rows per lane group: T <= 128 rows, at least 32 per pass of the workgroup
+    static_assert(4 * G::GPW * R >= 128, "the rows of a block fit the lane groups");
+    __shared__ float s_sum[4];
+    const Params &a = p.a;
+    const int nb = (a.start_pos + p.S + p.T - 1) >> p.t_shift;
+    const int blk = blockIdx.x % nb, bh = blockIdx.x / nb, b = bh / a.H, h = bh % a.H;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane / LPR, lig = lane % LPR, e0 = lig * 16;
+    const int ctx = a.start_pos + p.S, row0 = blk * p.T;
+    const bool has_chunk = !G::PADDED || lig < G::CH, open = row0 + p.T > ctx;
+    const float scale = a.scale * kLog2e, ks = open ? 1.f : p.k_scale[(size_t)bh * p.nblk + blk];
+    float k[R][16];
+    int row[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const int at = (j * 4 + wave) * G::GPW + g;
+        row[j] = at < p.T && row0 + at < ctx ? row0 + at : -1;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) k[j][i] = 0.f;
+        if (row[j] >= 0 && has_chunk) {
+            if (open) {
+                const _Float16 *t = p.k_tail + ((size_t)bh * p.T + at) * D + e0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) k[j][i] = (float)t[i];
+            } else {
+                const int8_t *t = p.k8 + ((size_t)bh * a.L + row[j]) * D + e0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) k[j][i] = (float)t[i];
+            }
+        }
+    }
+    float sum = 0.f;
+    for (int s = p.S - p.weight_queries; s < p.S; ++s) {
+        const int64_t token = (int64_t)b * p.S + s;
+        float q[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) q[i] = 0.f;
+        if (has_chunk) {
+            load_input<16>(a.q, p.in_kind, (size_t)(token * a.H + h) * D + e0, p.in_kind == kInI32 ? a.inp_scale[token] : 0.f,
+                           p.in_kind == kInI32 ? a.wq_scale + h * D + e0 : nullptr, q);
+            rotate_run<16>(q, a.freq_cis + (size_t)(a.rope_row < 0 ? a.start_pos + s : a.rope_row + s) * D + e0);
+        }
+        const float2 st = p.stats[(size_t)bh * p.S + s];
+        const float rl = st.y > 0.f ? 1.0f / st.y : 0.f;
+        float acc[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            acc[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[j] = fmaf(k[j][i], q[i], acc[j]);
+        }
+        group_sum_n<LPR, R>(acc);
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            if (row[j] < 0) continue;
+            const float mk = a.attn_mask ? a.attn_mask[(size_t)(a.start_pos + s) * a.mask_ld + row[j]] * kLog2e : 0.f;
+            const float e = __builtin_amdgcn_exp2f(fmaf(acc[j], ks * scale, mk) - st.x) * rl;
+            if (st.y > 0.f) sum += e;
+        }
+    }
+    sum = lig == 0 ? sum : 0.f;
+    sum = wave_sum(sum);
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        const float w = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        float *dst = p.weights + (size_t)bh * p.nblk + blk;
+        *dst = row0 >= a.start_pos ? w : *dst + w;
+    }
+}
+
+// ---------------------------------------------------------------- read-back
+
+// out_k, out_v [B,H,n,D] in O: integers * scale for complete blocks, the tail behind them, zeros behind a sequence's rows.
+// grid = B*H * 2 * groups (the groups of 1024 chunks of one (b,h) fastest), block = 256; a lane writes 16 bytes.  Bound by the traffic, D bytes in and
+// D * sizeof(O) out per row.
+template <typename O>
+__global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Params p, O *out_k, O *out_v, int n, int D, int groups)
+{
+    constexpr int VEC = 16 / (int)sizeof(O), NU = 4;
+    typedef O vec __attribute__((ext_vector_type(VEC)));
+    const int bh = blockIdx.x / groups >> 1, b = bh / p.a.H;
+    const bool is_v = (blockIdx.x / groups & 1) != 0;
+    int rows = p.a.pos_per_seq ? p.a.pos_per_seq[b] : n;
+    rows = min(rows, min(n, p.a.L)); // (a negative count: all zeros)
+    const int rows8 = rows > 0 ? rows & ~(p.T - 1) : 0;
+    const int8_t *src = (is_v ? p.v8 : p.k8) + (size_t)bh * p.a.L * D;
+    const _Float16 *tail = (is_v ? p.v_tail : p.k_tail) + (size_t)bh * p.T * D;
+    const float *scale = (is_v ? p.v_scale : p.k_scale) + (size_t)bh * p.nblk;
+    O *out = (is_v ? out_v : out_k) + (size_t)bh * n * D;
+    const uint32_t CPR = D / VEC, total = (uint32_t)n * CPR; // (n * D stays below 2^31)
+    const uint32_t i0 = (blockIdx.x % groups) * (256 * NU) + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const uint32_t i = i0 + u * 256;
+        if (i >= total) return;
+        const int row = (int)(i / CPR), e0 = (int)(i % CPR) * VEC;
+        vec y;
+        if (row < rows8) {
+            const float sc = scale[row >> p.t_shift];
+            uint32_t x[VEC / 4];
+            if constexpr (VEC == 8) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(src + (size_t)row * D + e0);
+                x[0] = v.x; x[1] = v.y;
+            } else {
+                x[0] = *reinterpret_cast<const uint32_t *>(src + (size_t)row * D + e0);
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y[j] = to_storage<O>(__fmul_rn((float)(int8_t)(x[j / 4] >> (8 * (j % 4))), sc));
+        } else if (row < rows) {
+            const _Float16 *t = tail + (size_t)(row - rows8) * D + e0;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y[j] = (O)t[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y[j] = (O)0;
+        }
+        *reinterpret_cast<vec *>(out + (size_t)i * VEC) = y;
+    }
+}
+
+// ---------------------------------------------------------------- eviction
+
+struct Kv8EvictParams {
+    const int8_t *k8, *v8;
+    const float *k_scale, *v_scale, *weights;
+    const _Float16 *k_tail, *v_tail;
+    int8_t *k8_to, *v8_to;
+    float *k_scale_to, *v_scale_to, *weights_to;
+    _Float16 *k_tail_to, *v_tail_to; // NULL: the tails stay where they are
+    int32_t *kept;                // [B*H, keep] source blocks in ascending order, -1 behind the last
+    int32_t *rows_to;             // [B]
+    const int32_t *rows_per_seq;  // [B] or NULL
+    int32_t rows, B, H, D, T, t_shift, nblk, nblk_to, keep, recent;
+};
+
+// Rows of sequence b before the eviction; -1 where the count lies outside the cache (nothing is moved then).
+__device__ __forceinline__ int evict_rows(const Kv8EvictParams &p, int b)
+{
+    const int r = p.rows_per_seq ? p.rows_per_seq[b] : p.rows;
+    return r < 0 || r > p.nblk * p.T ? -1 : r;
+}
+
+// Order-preserving unsigned image of a weight: larger weight, larger key; NaN below everything, -0 = +0.
+__device__ __forceinline__ uint32_t weight_key(float w)
+{
+    if (w != w) return 0u;
+    const uint32_t u = __float_as_uint(w + 0.f);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+// Exclusive prefix sum of a flag over the 256 threads; total: the number of flags set.
+__device__ __forceinline__ int block_rank(bool flag, int *s_cnt, int &total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned long long bal = __ballot(flag);
+    __syncthreads(); // s_cnt is free
+    if (lane == 0) s_cnt[wave] = __popcll(bal);
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) before += s_cnt[w];
+        total += s_cnt[w];
+    }
+    return before + __popcll(bal & ((1ull << lane) - 1ull));
+}
+
+// grid = B*H, block = 256.  Which blocks stay: the last `recent` and, of the rest, those of the largest weight, ties to the
+// lowest block.  The weight of the last one that stays is found by four passes over the bits of the keys, eight at a time
+// (a histogram in LDS each), so any number of blocks is served; the list is then written in ascending order, and scales and
+// weights move with it.  In place, an entry moves to its own or a lower slot: 256 entries are read before they are written.
+__global__ __launch_bounds__(256) static void kv8_select_kernel(const Kv8EvictParams p)
+{
+    __shared__ int s_hist[256];
+    __shared__ int s_cnt[4];
+    __shared__ uint32_t s_pick[2]; // threshold byte, entries still wanted at it
+    const int bh = blockIdx.x, b = bh / p.H, tid = threadIdx.x;
+    const int rows = evict_rows(p, b);
+    const int n = rows < 0 ? 0 : rows >> p.t_shift;
+    const int keep = min(p.keep, n), recent = min(p.recent, keep);
+    const int cand = n - recent, want = keep - recent; // the first `cand` blocks compete for `want` places
+    const float *w = p.weights + (size_t)bh * p.nblk;
+    uint32_t prefix = 0, mask = 0;
+    int left = want;
+    if (want > 0 && want < cand) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            s_hist[tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < cand; i += 256) {
+                const uint32_t k = weight_key(w[i]);
+                if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1);
+            }
+            __syncthreads();
+            if (tid < 64) { // the largest byte whose keys and all larger ones are enough: one wave, four bytes a lane
+                const int d3 = s_hist[255 - 4 * tid], d2 = s_hist[254 - 4 * tid], d1 = s_hist[253 - 4 * tid], d0 = s_hist[252 - 4 * tid];
+                int sum = d3 + d2 + d1 + d0, incl = sum;
+#pragma unroll
+                for (int o = 1; o < 64; o *= 2) {
+                    const int y = __shfl_up(incl, o);
+                    if (tid >= o) incl += y;
+                }
+                const int above = incl - sum;
+                if (above < left && incl >= left) {
+                    int byte = 255 - 4 * tid, at = above;
+                    if (at + d3 < left) { at += d3; --byte; if (at + d2 < left) { at += d2; --byte; if (at + d1 < left) { at += d1; --byte; } } }
+                    s_pick[0] = (uint32_t)byte;
+                    s_pick[1] = (uint32_t)(left - at);
+                }
+            }
+            __syncthreads();
+            prefix |= s_pick[0] << shift;
+            mask |= 255u << shift;
+            left = (int)s_pick[1];
+            __syncthreads();
+        }
+    }
+    // keys above `prefix` stay, and the first `left` equal to it
+    const bool all = want >= cand, none = want <= 0;
+    int *list = p.kept + (size_t)bh * p.keep;
+    int placed = 0, equal = 0;
+    for (int base = 0; base < n; base += 256) {
+        const int i = base + tid;
+        const uint32_t k = i < cand && !all && !none ? weight_key(w[i]) : 0u;
+        const bool tie = i < cand && !all && !none && k == prefix;
+        int n_tie;
+        const int tie_rank = equal + block_rank(tie, s_cnt, n_tie);
+        equal += n_tie;
+        const bool stay = i < n && (i >= cand || all || (!none && (k > prefix || (tie && tie_rank < left))));
+        int n_stay;
+        const int at = placed + block_rank(stay, s_cnt, n_stay);
+        float ws = 0.f, ksc = 0.f, vsc = 0.f;
+        if (stay) {
+            ws = w[i];
+            ksc = p.k_scale[(size_t)bh * p.nblk + i];
+            vsc = p.v_scale[(size_t)bh * p.nblk + i];
+        }
+        __syncthreads(); // read before any slot of this trip is written
+        if (stay) {
+            list[at] = i;
+            p.weights_to[(size_t)bh * p.nblk_to + at] = ws;
+            p.k_scale_to[(size_t)bh * p.nblk_to + at] = ksc;
+            p.v_scale_to[(size_t)bh * p.nblk_to + at] = vsc;
+        }
+        placed += n_stay;
+    }
+    for (int i = keep + tid; i < p.keep; i += 256) list[i] = -1;
+    if (tid == 0) {
+        const int open = rows < 0 ? 0 : rows & (p.T - 1);
+        if (open && keep < p.nblk_to) p.weights_to[(size_t)bh * p.nblk_to + keep] = w[n]; // the open block's weight
+        if (bh % p.H == 0) p.rows_to[b] = rows < 0 ? -1 : (keep << p.t_shift) + open;
+    }
+}
+
+// Moves the listed blocks: grid = B*H * 2 * slices of a block (fastest), block = 256.  A thread owns one 16-byte column of the block for
+// every block it moves, so in place nothing but its own column can stand in its way, and it moves the blocks in ascending
+// order, 8 of them read before the first is written (a block moves to its own or a lower slot).
+__global__ __launch_bounds__(256) static void kv8_move_kernel(const Kv8EvictParams p, int slices)
+{
+    constexpr int NB = 8;
+    const int bh = blockIdx.x / slices >> 1, b = bh / p.H, slice = blockIdx.x % slices;
+    const bool is_v = (blockIdx.x / slices & 1) != 0;
+    const int rows = evict_rows(p, b);
+    if (rows < 0) return;
+    const int keep = min(p.keep, rows >> p.t_shift);
+    const int col = slice * 256 + threadIdx.x, cols = p.T * p.D / 16;
+    const int *list = p.kept + (size_t)bh * p.keep;
+    if (col < cols) {
+        const u32x4 *src = reinterpret_cast<const u32x4 *>((is_v ? p.v8 : p.k8) + (size_t)bh * p.nblk * p.T * p.D) + col;
+        u32x4 *dst = reinterpret_cast<u32x4 *>((is_v ? p.v8_to : p.k8_to) + (size_t)bh * p.nblk_to * p.T * p.D) + col;
+        for (int r0 = 0; r0 < keep; r0 += NB) {
+            u32x4 x[NB];
+#pragma unroll
+            for (int u = 0; u < NB; ++u) x[u] = src[(size_t)list[min(r0 + u, keep - 1)] * cols];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < NB; ++u)
+                if (r0 + u < keep) dst[(size_t)(r0 + u) * cols] = x[u];
+        }
+    }
+    _Float16 *tail_to = is_v ? p.v_tail_to : p.k_tail_to;
+    if (tail_to && slice == 0) { // the open rows, into a cache with tails of its own
+        const half8 *src = reinterpret_cast<const half8 *>((is_v ? p.v_tail : p.k_tail) + (size_t)bh * p.T * p.D);
+        half8 *dst = reinterpret_cast<half8 *>(tail_to + (size_t)bh * p.T * p.D);
+        for (int i = threadIdx.x; i < (rows & (p.T - 1)) * (p.D / 8); i += 256) dst[i] = src[i];
+    }
+}
+
+} // namespace flattn

@@ -615,7 +615,7 @@ __device__ __forceinline__ uint32_t classify_ballots(bool open, bool nonzero, bo
 }
 
 // grid = (key tiles, query blocks), block = 256.
-__global__ __launch_bounds__(256) void prefill_mask_classify_kernel(const PrefillParams p, int NT)
+static __global__ __launch_bounds__(256) void prefill_mask_classify_kernel(const PrefillParams p, int NT)
 {
     __shared__ uint32_t s_cls[4];
     const int t = blockIdx.x, qb = blockIdx.y;
@@ -647,7 +647,7 @@ __global__ __launch_bounds__(256) void prefill_mask_classify_kernel(const Prefil
 // The same classes for a WHOLE mask [rows, cols] (row stride mask_ld), once per mask instead of once per call:
 // one byte per (32-key tile, 32-row block) at table[tile * table_ld + row block]; entries past the last row /
 // column repeat the last one.  grid = (ceil(cols/32), ceil(rows/32)), block = 64.
-__global__ __launch_bounds__(64) void mask_class_table_kernel(const float *mask, int64_t mask_ld, int rows, int cols,
+static __global__ __launch_bounds__(64) void mask_class_table_kernel(const float *mask, int64_t mask_ld, int rows, int cols,
                                                               uint8_t *table, int table_ld)
 {
     const int t = blockIdx.x, rb = blockIdx.y, lane = threadIdx.x;
@@ -1488,7 +1488,7 @@ __global__ __launch_bounds__(kWideWaves * 64) void prefill_attn_wide_kernel(cons
 // round trip, a reduction and a store per token, and its bandwidth is what is in flight (1024-thread workgroups,
 // two per compute unit, reached 3.1 TB/s).
 constexpr int kQuantThreads = 256;
-__global__ __launch_bounds__(kQuantThreads) void attn_quantize_transpose_kernel(const float *__restrict__ attn,
+static __global__ __launch_bounds__(kQuantThreads) void attn_quantize_transpose_kernel(const float *__restrict__ attn,
                                                                                 int8_t *__restrict__ out_q,
                                                                                 float *__restrict__ out_scale, int H, int S, int D)
 {

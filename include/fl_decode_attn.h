@@ -229,6 +229,80 @@ int fl_prefill_mask_classes_bytes(const fl_attn_desc *desc, size_t *bytes);
 int fl_prefill_mask_classify(const fl_attn_desc *desc, const float *attn_mask, int64_t mask_ld, void *classes,
                              size_t classes_bytes, void *hip_stream);
 
+/* ---- the 8-bit cache ------------------------------------------------------------------------------
+ * A cache of half the bytes of FL_ATTN_F16: K and V rows as signed bytes, one float scale per block of block_len
+ * consecutive rows and head.  No counterpart in the reference (its caches are FP32).  The rows of the block that
+ * is not full yet are kept in fp16 (rounded to nearest-even; non-finite values are stored as 0, finite ones kept
+ * within +-65504) and quantised together when the block's last row arrives: scale = absmax / 127, integer =
+ * rint(x * (127 / absmax)).  A row is therefore rounded to 8 bits once, and prompt pieces and decode steps may
+ * fill a block in any mix.  The rows of a block share a scale: rows nobody attends to (padding) should be zeros,
+ * large ones cost their block-mates' precision.
+ *
+ * The calls take fl_attn_desc and fl_attn_io as the calls above do: desc.dtype is the type of q/k_new/v_new (int32
+ * accumulators with qkv_inp_scale as before), io.k_cache / io.v_cache and desc.flags are ignored, everything else
+ * keeps its meaning — mask, positions, INT8 output, one launch after fl_kv8_workspace_init() with
+ * FL_ATTN_IO_WORKSPACE_READY.  Attention reads the cache as it stands after the append. */
+typedef struct fl_kv8_cache {
+    uint32_t struct_size; /* sizeof(fl_kv8_cache) */
+    int32_t block_len;    /* rows that share a scale: 32, 64 or 128; divides total_len (FL_ATTN_ERR_SHAPE) */
+    int8_t *k;            /* [B,H,L,D] */
+    int8_t *v;            /* same */
+    float *k_scale;       /* [B,H,L/block_len] */
+    float *v_scale;       /* same */
+    void *k_tail;         /* [B,H,block_len,D] fp16: row r of the open block at r % block_len; nothing behind the
+                             last row */
+    void *v_tail;         /* same */
+    float *weights;       /* NULL, or [B,H,L/block_len]: the softmax weight each block's rows have received.  A step
+                             adds to it; a block whose first row arrives in the call starts from 0.  A query all of
+                             whose keys are masked adds nothing */
+} fl_kv8_cache;
+
+/* Bytes of workspace for decode steps (seq_len 1) or for both decode steps and prompts of up to seq_len tokens. */
+int fl_kv8_workspace_bytes(const fl_attn_desc *desc, int32_t block_len, int32_t seq_len, size_t *bytes);
+
+/* Zeroes the arrival counters, once per workspace (see fl_decode_attn_workspace_init). */
+int fl_kv8_workspace_init(const fl_attn_desc *desc, int32_t block_len, int32_t seq_len, void *workspace,
+                          size_t workspace_bytes, void *hip_stream);
+
+/* One decode step: RoPE, append, attention over rows [0, start_pos].  rope_row_per_seq: NULL, or [B] table rows on the
+ * device in place of io.rope_row — after an eviction a sequence's next row is not its position. */
+int fl_kv8_decode_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io,
+                          const int32_t *rope_row_per_seq, void *hip_stream);
+
+/* The prompt phase (layouts and mask as fl_prefill_attn_forward).  With cache.weights, the last weight_queries queries
+ * of every sequence add theirs (0 = all); served for size_per_head <= 128 (FL_ATTN_ERR_HEAD_DIM). */
+int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io, int32_t seq_len,
+                           int32_t weight_queries, void *hip_stream);
+
+/* The values of rows [0, rows) as [B,H,rows,D] in desc.dtype: to move a sequence to another cache type, to look at one.
+ * rows_per_seq: NULL, or [B] on the device: rows from there on are zeros. */
+int fl_kv8_read(const fl_attn_desc *desc, const fl_kv8_cache *cache, int32_t rows, const int32_t *rows_per_seq,
+                void *k_out, void *v_out, void *hip_stream);
+
+/* Eviction by accumulated weight: of the n = rows / block_len complete blocks of every (b,h), the last recent_blocks
+ * stay, and of the others those of the largest weight (NaN last, ties to the earlier block), keep_blocks in all (all of
+ * them where n is smaller), in their order.  Rows, scales and weights move to the front of `to`, which is either the
+ * cache itself (the same pointers throughout) or another one that overlaps it nowhere.  The open block follows: its
+ * rows stay in the tail (or are copied to the other cache's), its weight moves to entry keep. */
+typedef struct fl_kv8_evict_args {
+    uint32_t struct_size;        /* sizeof(fl_kv8_evict_args) */
+    int32_t rows;                /* rows in the cache (= the next start_pos) */
+    const int32_t *rows_per_seq; /* NULL, or [B] on the device; a count outside [0, L] moves nothing: kept and
+                                    rows_out are -1 for that sequence */
+    int32_t keep_blocks;         /* >= 1, at most to_total_len / block_len */
+    int32_t recent_blocks;       /* 0 .. keep_blocks */
+    int32_t to_total_len;        /* rows per (b,h) of `to`; 0 = desc.total_len */
+    int32_t reserved;            /* 0 */
+    int32_t *kept;               /* [B,H,keep_blocks]: the blocks that stay, ascending, -1 behind the last */
+    int32_t *rows_out;           /* [B]: rows after the eviction */
+} fl_kv8_evict_args;
+int fl_kv8_evict(const fl_attn_desc *desc, const fl_kv8_cache *from, const fl_kv8_cache *to,
+                 const fl_kv8_evict_args *args, void *hip_stream);
+
+/* Bytes of one layer's K (or V) rows, scales and tail. */
+int fl_kv8_cache_bytes(const fl_attn_desc *desc, int32_t block_len, size_t *rows_bytes, size_t *scale_bytes,
+                       size_t *tail_bytes);
+
 /* RoPE table producer on the device: rows x D floats, row r = [cos(r*w_0), sin(r*w_0), ...],
  * w_i = base^(-2i/D).  Replaces launchPrecomputeFreqsCis (decoding_kernels.cu:85-135,
  * called at decoding_sampling.cu:190) with correctly rounded sincos instead of fast intrinsics. */

@@ -1,0 +1,468 @@
+"""The 8-bit key/value cache on the GPU, through the C ABI, against float64 (tests/kv8_reference.py).  Rows, scales and tails
+are compared bit for bit, whole arrays, so that a store outside its place shows; what has not been written yet holds NaN."""
+import numpy as np
+import pytest
+
+from fasterllama_amd import capi, synth
+import kv8_reference as kr
+
+pytestmark = pytest.mark.gpu
+
+NEG = -3.4028234663852886e38
+
+
+def to_gpu(c, dev):
+    import torch
+    from fasterllama_amd.kv8 import KV8Cache
+    return KV8Cache.of(c.T, *(torch.from_numpy(getattr(c, n).copy()).to(dev) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail")),
+                       weights=None if c.weights is None else torch.from_numpy(c.weights.copy()).to(dev))
+
+
+def bits(x):
+    return np.ascontiguousarray(x).view({1: np.uint8, 2: np.uint16, 4: np.uint32}[x.dtype.itemsize])
+
+
+def assert_cache(g, c, steps=1, rows=None):
+    """rows: of the cache after a prompt.  A prompt that completes a block need not take its rows through the tail, as single
+    steps do: behind the open block's rows a tail holds nothing."""
+    for n in c.names():
+        x, want = getattr(g, n).cpu().numpy(), getattr(c, n)
+        if rows is not None and n.endswith("_tail"):
+            x, want = x[:, :, :rows % c.T], want[:, :, :rows % c.T]
+        if n == "weights":
+            # a weight's relative error is that of the softmax (a few hundred U at the sizes here), per step
+            ok = ~np.isnan(want)
+            assert np.array_equal(np.isnan(x), ~ok), "weights: NaN elsewhere"
+            assert (np.abs(x[ok] - want[ok]) <= 2e-5 * steps * np.maximum(1.0, np.abs(want[ok]))).all(), np.abs(x[ok] - want[ok]).max()
+        else:
+            bad = np.flatnonzero(bits(x).ravel() != bits(want).ravel())
+            assert bad.size == 0, f"{n}: {bad.size} of {x.size} differ, first at {np.unravel_index(bad[0], x.shape)}"
+
+
+def assert_out(got, want, tol, what=""):
+    got = got.cpu().numpy().astype(np.float64).reshape(want.shape)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), f"{what}: NaN elsewhere"
+    err = np.where(np.isnan(want), 0.0, np.abs(got - want))
+    print(f"{what}: max error {err.max():.2e}, of the tolerance {np.max(err / np.maximum(tol, 1e-300)):.3f}")
+    assert (err <= tol).all(), f"{what}: {err.max()} against {np.max(tol)}"
+
+
+def inputs(B, S, H, D, dtype, seed):
+    r = np.random.RandomState(seed)
+    if dtype == "i32":
+        acc = [r.randint(-40000, 40000, (B, S, H, D)).astype(np.int32) for _ in range(3)]
+        sc = [(r.rand(B, S) * 2e-3 + 1e-4).astype(np.float32)] + [(r.rand(H * D) * 0.05 + 0.01).astype(np.float32) for _ in range(3)]
+        val = [((a.astype(np.float32) * sc[0][..., None, None]) * w.reshape(H, D)).astype(np.float32) for a, w in zip(acc, sc[1:])]
+        return acc, val, sc
+    x = [r.randn(B, S, H, D).astype(np.float16 if dtype == "f16" else np.float32) for _ in range(3)]
+    return x, x, None
+
+
+def masks(kind, L, seed=0):
+    i = np.arange(L)
+    if kind is None:
+        return None
+    if kind == "causal":
+        return np.where(i[None] > i[:, None], np.float32(NEG), np.float32(0)).astype(np.float32)
+    if kind == "inf_window":  # -inf outside the last 40 columns
+        return np.where((i[None] > i[:, None]) | (i[None] + 40 < i[:, None]), np.float32(-np.inf), np.float32(0)).astype(np.float32)
+    if kind == "soft":
+        return np.where(i[None] > i[:, None], np.float32(-1e5), np.random.RandomState(seed).randn(L, L)).astype(np.float32)
+    if kind == "strict":  # the first row sees nothing
+        return np.where(i[None] >= i[:, None], np.float32(NEG), np.float32(0)).astype(np.float32)
+    raise KeyError(kind)
+
+
+class Case:
+    def __init__(self, dev, B, H, D, L, T, dtype="f16", rows=0, weights=False, nsplit=0, max_seq_len=1, seed=0, scale=0.0):
+        import torch
+        from fasterllama_amd.kv8 import KV8Attention
+        self.dev, self.B, self.H, self.D, self.L, self.T, self.dtype, self.seed = dev, B, H, D, L, T, dtype, seed
+        self.scale = scale
+        self.rows = np.full(B, rows) if np.isscalar(rows) else np.asarray(rows)
+        self.ref = kr.Cache(B, H, D, L, T, weights, seed=seed).fill(np.clip(self.rows, 0, L - 1), seed + 1)
+        self.gpu = to_gpu(self.ref, dev)
+        self.table = synth.freq_cis_table(L + 64, D)
+        self.table_d = torch.from_numpy(self.table).to(dev)
+        self.op = KV8Attention(B, H, D, L, torch.float16 if dtype == "f16" else torch.float32, T, max_seq_len, nsplit, scale, dev)
+
+    def t(self, x):
+        import torch
+        return None if x is None else torch.from_numpy(np.ascontiguousarray(x)).to(self.dev)
+
+    def feed(self, S, seed):
+        raw, val, sc = inputs(self.B, S, self.H, self.D, self.dtype, seed)
+        return [self.t(x) for x in raw], val, None if sc is None else tuple(self.t(x) for x in sc)
+
+    def decode(self, mask=None, ragged=False, rope=None, seed=7, bound=None, **kw):
+        raw, val, sc = self.feed(1, seed)
+        if ragged:
+            kw.update(start_pos_per_seq=self.t(self.rows.astype(np.int32)), max_start_pos=int(self.rows.max()) if bound is None else bound)
+        else:
+            kw.update(start_pos=int(self.rows[0]))
+        if rope is not None:
+            kw.update(rope_row_per_seq=self.t(np.asarray(rope, np.int32)))
+        got = self.op.decode(*raw, self.gpu, self.table_d, attn_mask=self.t(mask), scales=sc, **kw)
+        start = self.rows if bound is None else np.where(self.rows > bound, -1, self.rows)
+        want, tol = self.ref.step(*val, self.table, start, mask, rope, self.scale)
+        return got, want[:, :, 0], tol[..., 0]
+
+    def prompt(self, S, mask=None, seed=9, weight_queries=0, **kw):
+        raw, val, sc = self.feed(S, seed)
+        got = self.op.prefill(*raw, self.gpu, self.table_d, start_pos=int(self.rows[0]), attn_mask=self.t(mask), scales=sc,
+                              weight_queries=weight_queries, **kw)
+        want, tol = self.ref.step(*val, self.table, self.rows, mask, None, self.scale, weight_queries)
+        return got, want, tol
+
+
+# ------------------------------------------------------------------------------------------------------------- decode
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 256, 512, 1024])
+@pytest.mark.parametrize("T", [32, 64, 128])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_decode_head_sizes(gpu, D, T, dtype):
+    for rows in (0, 1, T - 1, T, 2 * T + 5, 3 * T - 1):
+        c = Case(gpu, 2, 3, D, 3 * T if T == 128 else 4 * T, T, dtype, rows, weights=True)
+        got, want, tol = c.decode()
+        assert_out(got, want, tol, f"rows {rows}")
+        assert_cache(c.gpu, c.ref)
+
+
+@pytest.mark.parametrize("kind", ["causal", "inf_window", "soft"])
+@pytest.mark.parametrize("rows", [31, 63, 200, 383])
+@pytest.mark.parametrize("nsplit", [1, 3])
+def test_decode_masks(gpu, kind, rows, nsplit):
+    c = Case(gpu, 2, 2, 64, 512, 32, "f32", rows, weights=True, nsplit=nsplit)
+    got, want, tol = c.decode(masks(kind, 512))
+    assert_out(got, want, tol)
+    assert_cache(c.gpu, c.ref)
+
+
+@pytest.mark.parametrize("D,rows", [(128, 0), (96, 70)])
+def test_a_row_that_sees_nothing_is_nan_and_gathers_nothing(gpu, D, rows):
+    m = np.full((128, 128), NEG, np.float32)
+    for value in (NEG, -np.inf):
+        m[:] = value
+        c = Case(gpu, 1, 2, D, 128, 64, "f16", rows, weights=True)
+        before = c.ref.weights.copy()
+        got, want, tol = c.decode(m)
+        assert np.isnan(got.cpu().numpy()).all() and np.isnan(want).all()
+        after = c.gpu.weights.cpu().numpy()
+        n = rows // 64 + (rows % 64 > 0)
+        assert np.array_equal(after[:, :, :n], before[:, :, :n])
+
+
+@pytest.mark.parametrize("ready", [True, False])
+@pytest.mark.parametrize("nsplit", [0, 2, 7, 1024])
+def test_decode_splits(gpu, nsplit, ready):
+    c = Case(gpu, 1, 2, 128, 2048, 64, "f16", 2000, weights=True, nsplit=nsplit)
+    if not ready:  # two launches
+        def without(call, *args):
+            c.op.io.flags = 0
+            capi.check(call(*args, 0))
+        c.op._enqueue = without
+    import torch
+    torch.cuda.synchronize()
+    for step in range(2):  # the counters are zero again for the second
+        c.rows[:] = 2000 + step
+        got, want, tol = c.decode(seed=step)
+        torch.cuda.synchronize()
+        assert_out(got, want, tol)
+    assert_cache(c.gpu, c.ref, 2)
+
+
+def test_decode_from_an_empty_cache_over_block_borders(gpu):
+    c = Case(gpu, 2, 2, 96, 96, 32, "f16", 0, weights=True)
+    for step in range(96):
+        c.rows[:] = step
+        got, want, tol = c.decode(seed=100 + step)
+        assert_out(got, want, tol, f"step {step}")
+    assert_cache(c.gpu, c.ref, 96)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "i32"])
+@pytest.mark.parametrize("nsplit", [0, 4])
+def test_decode_ragged_with_positions_outside(gpu, dtype, nsplit):
+    rows = np.array([0, 511, 31, 600, -1, 63, 64, 200, 640, 450])
+    c = Case(gpu, 10, 3, 64, 640, 32, dtype, rows, weights=True, nsplit=nsplit)
+    got, want, tol = c.decode(ragged=True, bound=599, rope=np.array([5, 0, 1, 2, 3, 4, 5, 100, 7, 650]))
+    assert_out(got, want, tol)
+    assert np.isnan(got.cpu().numpy()[[3, 4, 8]]).all()
+    assert_cache(c.gpu, c.ref)
+
+
+def test_decode_scales_of_stale_blocks_and_rows_are_never_read(gpu):
+    """The whole cache behind the rows is NaN scales and random integers (Cache's junk): the last trip of a wave reaches over
+    the last complete block at head sizes whose trips are longer than a block."""
+    for D in (32, 64):
+        c = Case(gpu, 1, 1, D, 512, 32, "f16", 33, weights=True)
+        got, want, tol = c.decode()
+        assert_out(got, want, tol)
+
+
+def test_non_finite_inputs_do_not_spread(gpu):
+    """A NaN or infinity in a key or value is stored as 0; in a query it makes that head's output NaN."""
+    import torch
+    for rows in (10, 31):
+        c = Case(gpu, 1, 3, 64, 64, 32, "f32", rows)
+        raw, val, _ = c.feed(1, 3)
+        q, k, v = (x.copy() for x in val)
+        k[0, 0, 0, 5], k[0, 0, 1, 6], v[0, 0, 0, 7], v[0, 0, 2, 8] = np.nan, np.inf, -np.inf, 1e30
+        q[0, 0, 1, 3] = np.nan
+        got = c.op.decode(c.t(q), c.t(k), c.t(v), c.gpu, c.table_d, start_pos=rows)
+        want, tol = c.ref.step(q, k, v, c.table, c.rows)
+        assert np.isnan(got.cpu().numpy().reshape(3, 64)[1]).all()
+        assert_out(got.view(1, 3, 64)[:, [0]], want[:, [0], 0], tol[..., 0])
+        assert_cache(c.gpu, c.ref)
+
+
+def test_decode_int8_output_and_int32_input(gpu):
+    import torch
+    c = Case(gpu, 3, 4, 128, 256, 64, "i32", 190)
+    q8, sc = torch.zeros(3, 512, dtype=torch.int8, device=gpu), torch.zeros(3, device=gpu)
+    out = torch.empty(3, 512, device=gpu)
+    _, want, tol = c.decode(out=out, out_int8=q8, out_scale=sc)
+    assert_out(out, want, tol)
+    x = out.cpu().numpy()
+    top = np.abs(x).max(1)
+    assert np.array_equal(sc.cpu().numpy(), top / np.float32(127))
+    assert np.array_equal(q8.cpu().numpy(), np.rint((x * np.float32(127)) / top[:, None]).astype(np.int8))
+
+
+# ------------------------------------------------------------------------------------------------------------- prompt
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 256, 512, 1024])
+@pytest.mark.parametrize("T,dtype", [(32, "f32"), (64, "f16"), (128, "f16")])
+def test_prompt_head_sizes(gpu, D, T, dtype):
+    for start, S in ((0, 1), (0, T), (5, 2 * T), (T, 17), (T - 1, T + 2)):
+        c = Case(gpu, 2, 2, D, 4 * T, T, dtype, start, weights=D <= 128, max_seq_len=S)
+        got, want, tol = c.prompt(S, masks("causal", 4 * T))
+        assert_out(got, want, tol, f"start {start} S {S}")
+        assert_cache(c.gpu, c.ref, S, start + S)
+
+
+@pytest.mark.parametrize("kind", [None, "causal", "inf_window", "soft", "strict"])
+@pytest.mark.parametrize("start,S", [(0, 300), (77, 333), (64, 128), (130, 1)])
+def test_prompt_masks(gpu, kind, start, S):
+    c = Case(gpu, 1, 3, 128, 448, 64, "f16", start, weights=True, max_seq_len=S)
+    got, want, tol = c.prompt(S, masks(kind, 448), weight_queries=50)
+    assert_out(got, want, tol)
+    assert_cache(c.gpu, c.ref, S, start + S)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "i32"])
+def test_prompt_in_pieces_and_steps_leaves_the_same_bits(gpu, dtype):
+    """Rows, scales and tails do not depend on how the rows arrived."""
+    S, pieces = 150, (40, 24, 1, 64, 21)
+    for T in (32, 128):
+        one = Case(gpu, 2, 2, 64, 256, T, dtype, 0, max_seq_len=S)
+        raw, val, sc = one.feed(S, 5)
+        one.op.prefill(*raw, one.gpu, one.table_d, scales=sc)
+        two = Case(gpu, 2, 2, 64, 256, T, dtype, 0, max_seq_len=S)
+        at = 0
+        for n in pieces:
+            part = [x[:, at:at + n].contiguous() for x in raw]
+            psc = None if sc is None else (sc[0][:, at:at + n].contiguous(), *sc[1:])
+            if n == 1:
+                two.op.decode(*part, two.gpu, two.table_d, start_pos=at, scales=psc)
+            else:
+                two.op.prefill(*part, two.gpu, two.table_d, start_pos=at, scales=psc)
+            at += n
+        one.ref.step(*val, one.table, [0, 0])
+        for c in (one, two):
+            for n in ("k", "v", "k_scale", "v_scale"):
+                m = 150 // T * (T if n in ("k", "v") else 1)
+                assert np.array_equal(bits(getattr(c.gpu, n).cpu().numpy()[:, :, :m]), bits(getattr(one.ref, n)[:, :, :m])), n
+            for n in ("k_tail", "v_tail"):
+                assert np.array_equal(bits(getattr(c.gpu, n).cpu().numpy()[:, :, :150 % T]), bits(getattr(one.ref, n)[:, :, :150 % T])), n
+
+
+def test_prompt_scores_of_every_size(gpu):
+    """Keys and queries of very different sizes, block to block: the scales and the running maximum have to keep up."""
+    c = Case(gpu, 1, 2, 128, 512, 32, "f32", 0, max_seq_len=400, weights=True)
+    raw, val, _ = c.feed(400, 3)
+    r = np.random.RandomState(0)
+    q, k, v = (x.copy() for x in val)
+    k *= np.exp2(r.randint(-6, 4, (1, 400, 1, 1))).astype(np.float32)
+    v *= np.exp2(r.randint(-12, 8, (1, 400 // 16, 1, 1)).repeat(16, 1)).astype(np.float32)
+    q *= np.exp2(r.randint(-4, 3, (1, 400, 1, 1))).astype(np.float32)
+    m = masks("causal", 512)
+    got = c.op.prefill(c.t(q), c.t(k), c.t(v), c.gpu, c.table_d, attn_mask=c.t(m))
+    want, tol = c.ref.step(q, k, v, c.table, c.rows, m)
+    assert_out(got, want, tol)
+    assert_cache(c.gpu, c.ref, 400, 400)
+
+
+def test_prompt_with_a_persistent_class_table_and_int8_output(gpu):
+    import torch
+    from fasterllama_amd.decode_attn import PrefillAttention
+    c = Case(gpu, 2, 3, 128, 512, 64, "f16", 96, max_seq_len=300)
+    m = masks("causal", 512)
+    md = c.t(m)
+    table = PrefillAttention(2, 3, 128, 512, 300, torch.float16, device=gpu).classify_mask(md)
+    q8, sc = torch.zeros(2, 300, 384, dtype=torch.int8, device=gpu), torch.zeros(2, 300, device=gpu)
+    out = torch.empty(2, 3, 300, 128, device=gpu)
+    _, want, tol = c.prompt(300, m, mask_tile_classes=table, out=out, out_int8=q8, out_scale=sc)
+    assert_out(out, want, tol)
+    x = out.cpu().numpy().transpose(0, 2, 1, 3).reshape(2, 300, 384)
+    top = np.abs(x).max(-1)
+    assert np.array_equal(sc.cpu().numpy(), top / np.float32(127))
+    assert np.array_equal(q8.cpu().numpy(), np.rint((x * np.float32(127)) / top[..., None]).astype(np.int8))
+
+
+# --------------------------------------------------------------------------------------------------------- read, evict
+
+@pytest.mark.parametrize("D,T,dtype", [(32, 32, "f32"), (96, 64, "f16"), (128, 128, "f32"), (1024, 32, "f16")])
+def test_read(gpu, D, T, dtype):
+    rows = np.array([0, 1, T, T + 3, 2 * T + T // 2, 3 * T])
+    c = Case(gpu, 6, 2, D, 3 * T, T, dtype, np.minimum(rows, 3 * T - 1))
+    rows = c.rows
+    for n in (1, T + 1, 3 * T):
+        for ragged in (True, False):
+            lens = np.minimum(rows if ragged else np.full(6, n), n)
+            if not ragged and n > rows.min():
+                continue
+            k, v = c.op.read(c.gpu, n, c.t(rows.astype(np.int32)) if ragged else None)
+            for b in range(6):
+                for x, want in zip((k, v), c.ref.values(b, int(lens[b]))):
+                    x = x[b].cpu().numpy()
+                    assert not x[:, lens[b]:].any()
+                    want = want.astype(np.float32).astype(x.dtype)
+                    # (the fp16 value is that of the 32-bit product)
+                    assert np.array_equal(x[:, :lens[b]], want)
+
+
+@pytest.mark.parametrize("D,T", [(32, 32), (96, 32), (128, 64), (256, 128)])
+@pytest.mark.parametrize("keep,recent", [(1, 0), (3, 3), (5, 2), (7, 1), (9, 4)])
+def test_evict(gpu, D, T, keep, recent):
+    L = 9 * T
+    rows = np.array([0, 3 * T, 7 * T + 5, 9 * T - 1, T - 1, -1, 9 * T + 1])
+    for place in ("in place", "same size", "smaller"):
+        c = Case(gpu, 7, 2, D, L, T, "f16", rows, weights=True)
+        r = np.random.RandomState(keep)
+        w = c.ref.weights
+        w[:] = r.randint(0, 4, w.shape)  # ties
+        w[0, 0, 1], w[2, 1, 3], w[3, 0, :] = np.nan, np.nan, np.inf
+        w[3, 1, :] = -0.0
+        w[3, 1, 2::3] = 0.0
+        c.gpu = to_gpu(c.ref, gpu)
+        into = None if place == "in place" else kr.Cache(7, 2, D, L if place == "same size" else keep * T, T, True, seed=5)
+        to = None if into is None else to_gpu(into, gpu)
+        kept, after = c.op.evict(c.gpu, keep, recent, 0, c.t(rows.astype(np.int32)), into=to)
+        want_kept, want_after = kr.evict(c.ref, rows, keep, recent, into)
+        assert np.array_equal(kept.cpu().numpy(), want_kept), (kept.cpu().numpy() != want_kept).any(-1)
+        assert np.array_equal(after.cpu().numpy(), want_after)
+        g, want = (c.gpu, c.ref) if into is None else (to, into)
+        for n in want.names():
+            assert np.array_equal(bits(getattr(g, n).cpu().numpy()), bits(getattr(want, n))), (place, n)
+
+
+def test_evict_many_blocks(gpu):
+    """More blocks than threads: weights over 30 binary orders, and all but equal ones."""
+    for spread in (True, False):
+        c = Case(gpu, 2, 2, 32, 32 * 1500, 32, "f16", 0, weights=True)
+        r = np.random.RandomState(1)
+        c.ref.weights[:] = np.exp2(r.uniform(-15, 15, c.ref.weights.shape)) if spread else 1.0 + r.randint(0, 3, c.ref.weights.shape) * 2.0 ** -23
+        c.ref.k_scale[:], c.ref.v_scale[:] = r.rand(*c.ref.k_scale.shape), r.rand(*c.ref.k_scale.shape)
+        c.gpu = to_gpu(c.ref, gpu)
+        rows = np.full(2, 32 * 1500)
+        kept, after = c.op.evict(c.gpu, 700, 100, 32 * 1500)
+        want_kept, want_after = kr.evict(c.ref, rows, 700, 100)
+        assert np.array_equal(kept.cpu().numpy(), want_kept)
+        assert_cache(c.gpu, c.ref)
+
+
+@pytest.mark.parametrize("T", [32, 64])
+def test_serving_run(gpu, T):
+    """Prompt, steps, eviction in place, steps: as a server would, with the budget of a small cache."""
+    L = 8 * T
+    c = Case(gpu, 2, 3, 64, L, T, "f16", 0, weights=True, max_seq_len=7 * T)
+    m = masks("causal", L)
+    got, want, tol = c.prompt(6 * T + 7, m, weight_queries=33)
+    assert_out(got, want, tol, "prompt")
+    rows, pos, steps = 6 * T + 7, 6 * T + 7, 33
+    for step in range(4 * T):
+        if rows == L:
+            # the weights decide as they stand here: those of the GPU and of the reference differ in their last bits
+            c.ref.weights[:] = c.gpu.weights.cpu().numpy()
+            kept, after = c.op.evict(c.gpu, 5, 2, rows)
+            want_kept, _ = kr.evict(c.ref, np.full(2, rows), 5, 2)
+            assert np.array_equal(kept.cpu().numpy(), want_kept)
+            rows = 5 * T
+            assert (after.cpu().numpy() == rows).all()
+        c.rows[:] = rows
+        got, want, tol = c.decode(seed=1000 + step, rope=[pos, pos]) if step % 2 else c.decode(seed=1000 + step, rope=[pos, pos], ragged=True)
+        assert_out(got, want, tol, f"step {step} row {rows}")
+        rows, pos, steps = rows + 1, min(pos + 1, L + 63), steps + 1
+    assert_cache(c.gpu, c.ref, steps)
+
+
+# ---------------------------------------------------------------------------------------------- streams, graphs, limits
+
+def test_side_stream_and_graph_replays(gpu):
+    """A captured step, replayed with eager work between: every replay equals the eager result."""
+    import torch
+    c = Case(gpu, 1, 4, 128, 2048, 64, "f16", 1983, weights=True)  # a split context, a block filled
+    m = c.t(masks("causal", 2048))
+    raw, _, _ = c.feed(1, 3)
+    start = to_gpu(c.ref, gpu)
+    names = c.ref.names()
+    side = torch.cuda.Stream(gpu)
+    side.wait_stream(torch.cuda.current_stream(gpu))
+    with torch.cuda.stream(side):
+        want = c.op.decode(*raw, c.gpu, c.table_d, start_pos=1983, attn_mask=m).clone()
+        want_state = {n: getattr(c.gpu, n).clone() for n in names}
+    side.synchronize()
+
+    def restore():
+        for n in names:
+            getattr(c.gpu, n).copy_(getattr(start, n))
+    restore()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = c.op.decode(*raw, c.gpu, c.table_d, start_pos=1983, attn_mask=m)
+    for _ in range(4):
+        restore()
+        out.fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        for n in names:
+            assert torch.equal(getattr(c.gpu, n).float().nan_to_num(7.0), want_state[n].float().nan_to_num(7.0)), n
+
+
+def test_caches_past_four_gib(gpu):
+    """Offsets of whole caches pass 32 bits: 2 x 4.3 GB of bytes, the last sequence's last rows."""
+    import torch
+    from fasterllama_amd.kv8 import KV8Attention, KV8Cache
+    B, H, D, L, T = 2, 1, 128, 128 * 131200, 128  # a slice of 2.15e9 bytes is beyond the limit: see the refusal
+    with pytest.raises(capi.FlAttnError):
+        KV8Attention(B, H, D, L, torch.float16, T, device=gpu)
+    B, L = 33, 128 * 8192  # 33 * 134 MB
+    op, cache = KV8Attention(B, H, D, L, torch.float16, T, device=gpu), KV8Cache(B, H, D, L, T, weights=True, device=gpu)
+    r = np.random.RandomState(0)
+    for b in (0, B - 1):
+        cache.k[b, 0, -256:-128] = torch.from_numpy(r.randint(-127, 128, (128, D)).astype(np.int8)).to(gpu)
+        cache.v[b, 0, -256:-128] = torch.from_numpy(r.randint(-127, 128, (128, D)).astype(np.int8)).to(gpu)
+        cache.k_scale[b, 0, -2], cache.v_scale[b, 0, -2] = 0.03, 0.02
+        cache.k_tail[b], cache.v_tail[b] = (torch.from_numpy(r.randn(1, T, D).astype(np.float16)).to(gpu) for _ in range(2))
+    mask = torch.full((1, L), NEG, device=gpu)
+    mask[:, -256:] = 0
+    table = torch.zeros(2, D, device=gpu)
+    table[:, 0::2] = 1
+    x = [torch.from_numpy(r.randn(B, 1, H, D).astype(np.float16)).to(gpu) for _ in range(3)]
+    pos = torch.full((B,), -1, dtype=torch.int32, device=gpu)
+    pos[[0, B - 1]] = L - 1
+    got = op.decode(*x, cache, table, attn_mask=mask, start_pos_per_seq=pos, max_start_pos=L - 1, rope_row_per_seq=pos * 0)
+    torch.cuda.synchronize()
+    for b in (0, B - 1):
+        small = kr.Cache(1, 1, D, 256, T, seed=1)
+        for n in ("k", "v"):
+            getattr(small, n)[0, :, :128] = getattr(cache, n)[b, :, -256:-128].cpu().numpy()
+            getattr(small, n + "_scale")[0, :, 0] = getattr(cache, n + "_scale")[b, :, -2].cpu().numpy()
+            getattr(small, n + "_tail")[0] = getattr(cache, n + "_tail")[b].cpu().numpy()
+        want, tol = small.step(*(t[[b]].cpu().numpy() for t in x), table.cpu().numpy(), [255], rope=[0])
+        assert_out(got[[b]], want[:, :, 0].reshape(1, D), tol.reshape(1, 1))
+        assert np.array_equal(cache.k[b, 0, -128:].cpu().numpy(), small.k[0, 0, 128:])
+    assert np.isnan(got[1:B - 1].cpu().numpy()).all()
