@@ -9,12 +9,14 @@
 #include "../../include/fl_decode_attn.h"
 #include "capi_common.hpp"
 #include "kv8_kernels.hpp"
+#include "kv8_prefill_kernels.hpp"
 
 namespace {
 
 using namespace flhost;
 using flattn::Kv8EvictParams;
 using flattn::Kv8Params;
+using flattn::Kv8PromptParams;
 
 constexpr size_t kCacheMinBytes = offsetof(fl_kv8_cache, weights) + sizeof(void *);
 constexpr size_t kEvictMinBytes = offsetof(fl_kv8_evict_args, rows_out) + sizeof(void *);
@@ -82,10 +84,10 @@ void make_plan(const fl_attn_desc *d, int ctx, bool ragged, fl_attn_plan *plan)
     plan->two_pass = plan->nsplit <= 1 ? 0 : ((int64_t)plan->nsplit * d->batch_size * d->head_num <= 4 * (int64_t)device_cus() ? 2 : 1);
 }
 
-// Workspace: [arrivals B*H] [float output B*H*S*D] [part_o] [part_m] [part_l] [granules] [mask tile classes] [statistics
-// B*H*S]; 256-byte sections.
+// Workspace: [arrivals B*H] [float output B*H*S*D] [part_o] [part_m] [part_l] [granules] [mask tile classes], and for the
+// block weights of a prompt [statistics B*H*S] [query operands] [query factors]; 256-byte sections.
 struct Layout {
-    size_t arrivals, tmp_out, part_o, part_m, part_l, granules, tile_class, stats, total;
+    size_t arrivals, tmp_out, part_o, part_m, part_l, granules, tile_class, stats, q_pairs, q_factor, total;
 };
 
 Layout layout(const fl_attn_desc *d, int S)
@@ -103,7 +105,10 @@ Layout layout(const fl_attn_desc *d, int S)
     w.part_l = take(slots * 4);
     w.granules = take(bh * (size_t)(d->total_len / granule_rows(d->size_per_head)) * 8);
     w.tile_class = take(qblocks * ktiles * 4);
-    w.stats = take(bh * (size_t)S * 8);
+    const size_t S32 = ((size_t)S + 31) / 32 * 32;
+    w.stats = take(bh * S32 * 8);
+    w.q_pairs = take(D <= 128 ? bh * S32 * D * 4 : 0);
+    w.q_factor = take(bh * S32 * 4);
     w.total = at;
     return w;
 }
@@ -175,20 +180,32 @@ hipError_t launch_append(const Kv8Params &p, hipStream_t stream)
 }
 
 template <int D>
-hipError_t launch_prompt(const Kv8Params &p, hipStream_t stream)
+hipError_t launch_prompt(const Kv8PromptParams &pp, hipStream_t stream)
 {
+    const Kv8Params &p = pp.k;
     hipError_t e = launch_append<D>(p, stream);
     if (e != hipSuccess) return e;
-    const dim3 grid((unsigned)(p.a.B * p.S) * (unsigned)p.a.H), block(flattn::kKv8Waves * 64);
-    e = p.a.attn_mask ? launch(flattn::kv8_attn_kernel<D, true, true>, grid, block, stream, p)
-                      : launch(flattn::kv8_attn_kernel<D, false, true>, grid, block, stream, p);
-    if constexpr (D <= 128) {
-        if (e == hipSuccess && p.stats) {
-            const unsigned nb = (unsigned)((p.a.start_pos + p.S + p.T - 1) / p.T);
-            e = launch(flattn::kv8_prompt_weights_kernel<D>, dim3(nb * (unsigned)(p.a.B * p.a.H)), block, stream, p);
+    const unsigned bh = (unsigned)(p.a.B * p.a.H);
+    if constexpr (D > 128) { // the matrix-core kernel's state no longer fits: one workgroup per query
+        const dim3 grid((unsigned)p.S * bh), block(flattn::kKv8Waves * 64);
+        if (p.a.attn_mask) return launch(flattn::kv8_attn_kernel<D, true, true>, grid, block, stream, p);
+        return launch(flattn::kv8_attn_kernel<D, false, true>, grid, block, stream, p);
+    } else {
+        const unsigned qblocks = (unsigned)((p.S + flattn::kPrefillQueriesPerBlock - 1) / flattn::kPrefillQueriesPerBlock);
+        if (p.a.attn_mask && !pp.f.class_table) { // no table of the whole mask at hand: classify the rows of this call
+            const int ktiles = (p.a.start_pos + p.S + flattn::kPrefillKeysPerStep - 1) / flattn::kPrefillKeysPerStep;
+            e = launch(flattn::prefill_mask_classify_kernel, dim3((unsigned)ktiles, qblocks), dim3(256), stream, pp.f, ktiles);
+            if (e != hipSuccess) return e;
         }
+        const dim3 grid(qblocks * bh), block(256);
+        e = p.a.attn_mask ? launch(flattn::kv8_prefill_attn_kernel<D, true>, grid, block, stream, pp)
+                          : launch(flattn::kv8_prefill_attn_kernel<D, false>, grid, block, stream, pp);
+        if (e != hipSuccess || !p.stats) return e;
+        const dim3 wgrid((unsigned)((p.a.start_pos + p.S + p.T - 1) / p.T) * bh);
+        if (p.T == 32) return launch(flattn::kv8_prompt_weights_kernel<D, 32>, wgrid, block, stream, pp);
+        if (p.T == 64) return launch(flattn::kv8_prompt_weights_kernel<D, 64>, wgrid, block, stream, pp);
+        return launch(flattn::kv8_prompt_weights_kernel<D, 128>, wgrid, block, stream, pp);
     }
-    return e;
 }
 
 #define KV8_BY_HEAD_SIZE(D, F, ...)                    \
@@ -204,7 +221,7 @@ hipError_t launch_prompt(const Kv8Params &p, hipStream_t stream)
     }
 
 hipError_t dispatch_decode(int D, const Kv8Params &p, const fl_attn_plan &plan, hipStream_t s) { KV8_BY_HEAD_SIZE(D, launch_decode, p, plan, s) }
-hipError_t dispatch_prompt(int D, const Kv8Params &p, hipStream_t s) { KV8_BY_HEAD_SIZE(D, launch_prompt, p, s) }
+hipError_t dispatch_prompt(int D, const Kv8PromptParams &p, hipStream_t s) { KV8_BY_HEAD_SIZE(D, launch_prompt, p, s) }
 #undef KV8_BY_HEAD_SIZE
 
 __global__ static void kv8_fill_zero_kernel(int32_t *dst, int64_t n)
@@ -347,12 +364,27 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
     Kv8Params p = make_params(desc, &c, &io);
     p.a.out = io.out ? io.out : reinterpret_cast<float *>(ws + w.tmp_out);
     p.S = seq_len;
+    Kv8PromptParams pp{};
+    flattn::PrefillParams &f = pp.f;
+    f.attn_mask = io.attn_mask; f.mask_ld = io.mask_ld;
+    f.tile_class = reinterpret_cast<uint32_t *>(ws + w.tile_class);
+    f.B = desc->batch_size; f.H = desc->head_num; f.L = L; f.S = seq_len; f.start_pos = io.start_pos;
+    if (io.mask_tile_classes && io.attn_mask && io.mask_ld >= L && io.start_pos % 32 == 0) {
+        if ((reinterpret_cast<uintptr_t>(io.mask_tile_classes) & 3u) != 0) return FL_ATTN_ERR_ALIGNMENT; // read a word at a time
+        f.class_table = static_cast<const uint8_t *>(io.mask_tile_classes);
+        f.class_ld = (int32_t)class_table_ld(L);
+    }
     if (c.weights) {
         p.stats = reinterpret_cast<float2 *>(ws + w.stats);
         p.weight_queries = weight_queries > 0 && weight_queries < seq_len ? weight_queries : seq_len;
+        pp.q_pairs = reinterpret_cast<flattn::half8 *>(ws + w.q_pairs);
+        pp.q_factor = reinterpret_cast<float *>(ws + w.q_factor);
+        pp.first_block = (seq_len - p.weight_queries) / 32;
+        pp.kept_blocks = (seq_len + 31) / 32 - pp.first_block;
     }
+    pp.k = p;
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
-    if (!check_hip(dispatch_prompt(D, p, stream))) return FL_ATTN_ERR_HIP;
+    if (!check_hip(dispatch_prompt(D, pp, stream))) return FL_ATTN_ERR_HIP;
     if (io.out_int8 && !check_hip(launch(flattn::attn_quantize_transpose_kernel, dim3((unsigned)(desc->batch_size * seq_len)), dim3(flattn::kQuantThreads),
                                          stream, p.a.out, io.out_int8, io.out_scale, desc->head_num, seq_len, D)))
         return FL_ATTN_ERR_HIP;

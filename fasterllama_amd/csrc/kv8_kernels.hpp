@@ -572,10 +572,7 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
         if (direct) a.out[(PROMPT ? (size_t)bh * p.S + s_query : (size_t)bh) * D + d] = O / Lsum;
         else store_partial<true>(a.part_o + slot * D + d, O);
     }
-    if (PROMPT) {
-        if (p.stats && tid == 0) p.stats[(size_t)bh * p.S + s_query] = make_float2(M, Lsum);
-        return;
-    }
+    if (PROMPT) return;
     if (direct) {
         if (gather) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -700,84 +697,6 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(const Kv8Params p)
             const int row = r0 + i / CPR, e0 = (i % CPR) * 8;
             *reinterpret_cast<half8 *>(tail + (size_t)(row - last * T) * D + e0) = new_chunk(row, e0);
         }
-    }
-}
-
-// ---------------------------------------------------------------- prompt phase: block weights
-
-// weights[b,h,blk] (+)= sum over the last weight_queries queries and the block's rows of e^(s - M) / sum, with the statistics
-// the attention kernel left.  grid = blocks * B*H, block = 256; a lane group owns up to four rows of the block.
-template <int D>
-__global__ __launch_bounds__(256) void kv8_prompt_weights_kernel(const Kv8Params p)
-{
-    typedef Kv8Geometry<D> G;
-    constexpr int LPR = G::LPR, R = 4; // rows per lane group: T <= 128 rows, at least 32 per pass of the workgroup
-    static_assert(4 * G::GPW * R >= 128, "the rows of a block fit the lane groups");
-    __shared__ float s_sum[4];
-    const Params &a = p.a;
-    const int nb = (a.start_pos + p.S + p.T - 1) >> p.t_shift;
-    const int blk = blockIdx.x % nb, bh = blockIdx.x / nb, b = bh / a.H, h = bh % a.H;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane / LPR, lig = lane % LPR, e0 = lig * 16;
-    const int ctx = a.start_pos + p.S, row0 = blk * p.T;
-    const bool has_chunk = !G::PADDED || lig < G::CH, open = row0 + p.T > ctx;
-    const float scale = a.scale * kLog2e, ks = open ? 1.f : p.k_scale[(size_t)bh * p.nblk + blk];
-    float k[R][16];
-    int row[R];
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        const int at = (j * 4 + wave) * G::GPW + g;
-        row[j] = at < p.T && row0 + at < ctx ? row0 + at : -1;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) k[j][i] = 0.f;
-        if (row[j] >= 0 && has_chunk) {
-            if (open) {
-                const _Float16 *t = p.k_tail + ((size_t)bh * p.T + at) * D + e0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) k[j][i] = (float)t[i];
-            } else {
-                const int8_t *t = p.k8 + ((size_t)bh * a.L + row[j]) * D + e0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) k[j][i] = (float)t[i];
-            }
-        }
-    }
-    float sum = 0.f;
-    for (int s = p.S - p.weight_queries; s < p.S; ++s) {
-        const int64_t token = (int64_t)b * p.S + s;
-        float q[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) q[i] = 0.f;
-        if (has_chunk) {
-            load_input<16>(a.q, p.in_kind, (size_t)(token * a.H + h) * D + e0, p.in_kind == kInI32 ? a.inp_scale[token] : 0.f,
-                           p.in_kind == kInI32 ? a.wq_scale + h * D + e0 : nullptr, q);
-            rotate_run<16>(q, a.freq_cis + (size_t)(a.rope_row < 0 ? a.start_pos + s : a.rope_row + s) * D + e0);
-        }
-        const float2 st = p.stats[(size_t)bh * p.S + s];
-        const float rl = st.y > 0.f ? 1.0f / st.y : 0.f;
-        float acc[R];
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            acc[j] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[j] = fmaf(k[j][i], q[i], acc[j]);
-        }
-        group_sum_n<LPR, R>(acc);
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            if (row[j] < 0) continue;
-            const float mk = a.attn_mask ? a.attn_mask[(size_t)(a.start_pos + s) * a.mask_ld + row[j]] * kLog2e : 0.f;
-            const float e = __builtin_amdgcn_exp2f(fmaf(acc[j], ks * scale, mk) - st.x) * rl;
-            if (st.y > 0.f) sum += e;
-        }
-    }
-    sum = lig == 0 ? sum : 0.f;
-    sum = wave_sum(sum);
-    if (lane == 0) s_sum[wave] = sum;
-    __syncthreads();
-    if (tid == 0) {
-        const float w = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-        float *dst = p.weights + (size_t)bh * p.nblk + blk;
-        *dst = row0 >= a.start_pos ? w : *dst + w;
     }
 }
 

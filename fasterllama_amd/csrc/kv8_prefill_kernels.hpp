@@ -1,0 +1,547 @@
+// Prompt phase over the 8-bit cache on the matrix cores (size_per_head 32, 64, 96, 128).
+//
+// Same shape as the fp16 caches' kernel: a workgroup owns 128 queries of one (b,h), 32 per wave, and walks the keys 32 at a
+// time through LDS; S^T = K Q^T leaves 16 probabilities of one query in every lane, in the operand layout of O^T = V^T P^T.
+// What the 8 bits change:
+//   operands   a byte is an exact fp16 number, so K and V enter v_mfma_f32_32x32x16_f16 as they are stored and the block's
+//              scale (uniform over a 32-key tile) stays outside: K's multiplies the score where the softmax scale does, V's
+//              goes into the exponent of the weight, e^(s - m) * vs / vref = 2^(s' - m' + log2(vs / vref)), and costs nothing
+//              per score either;
+//   precision  queries and weights are fp16 PAIRS, value + remainder (22 bits), twice the matrix instructions of single
+//              values, so that the output keeps the accuracy of 32-bit arithmetic (2e-7 of the result at the 7B shapes;
+//              weights rounded once to fp16 would leave 1.4e-4).  A query is scaled by a power of two so that its largest
+//              element lies in [256, 512), a weight by 2^7: remainders stay clear of fp16's smallest steps;
+//   loads      a tile is half the bytes: one 16-byte chunk of K and of V per thread (D = 128), widened to fp16 on the way
+//              into LDS by all four waves together.
+#pragma once
+
+#include "kv8_kernels.hpp"
+
+#pragma clang fp contract(off)
+
+namespace flattn {
+
+constexpr float kKv8WeightExp = 7.0f; // weights enter the second product times 2^7; kLazyMax = 8 more stay below 65504
+
+struct Kv8PromptParams {
+    Kv8Params k;
+    PrefillParams f;      // mask, tile classes, B, H, L, S, start_pos
+    half8 *q_pairs;       // workspace: rotated query operands of the last queries, for the block weights; or NULL
+    float *q_factor;      // [B*H, query blocks of 32, 32] with them
+    int32_t first_block;  // 32-query blocks from here on are kept
+    int32_t kept_blocks;
+};
+
+// Four signed bytes as fp16: 1024 + (b ^ 128) is the fp16 with that low byte, minus 1152 leaves b, exactly.
+__device__ __forceinline__ void widen4(uint32_t x, half2v &lo, half2v &hi)
+{
+    const uint32_t u = x ^ 0x80808080u;
+    const half2v off = {(_Float16)-1152.f, (_Float16)-1152.f};
+    lo = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off;
+    hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off;
+}
+
+__device__ __forceinline__ void wave_lds_sync() // orders this wave's LDS writes and reads
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <int D, bool HAS_MASK>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 8)))
+void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
+{
+    constexpr int BN = kPrefillKeysPerStep; // 32
+    constexpr int LDK = D + 8;                       // halfs; rows start 4 banks apart (128-bit operand reads)
+    constexpr int LDV = D == 96 ? D + 48 : D + 32;   // halfs; for the transposing reads, as the fp16 caches' kernel
+    constexpr int NC = D / 16, NDT = D / 32;
+    constexpr int NCH = BN * D / 16;                 // 16-byte chunks of a byte tile
+    constexpr int LPT = (2 * NCH + 255) / 256;       // chunks per thread: K's first, then V's
+    constexpr int CPR8 = D / 16;                     // chunks per row
+    constexpr int LDQ = D + 8, HALF_D = D >= 128 ? 64 : 32, LDO = HALF_D + 4;
+    constexpr int TILE_HALFS = 2 * BN * (LDK + LDV), Q_HALFS = kPrefillQueriesPerBlock * LDQ, O_HALFS = kPrefillQueriesPerBlock * LDO * 2;
+    constexpr int SMEM_HALFS = TILE_HALFS > Q_HALFS ? (TILE_HALFS > O_HALFS ? TILE_HALFS : O_HALFS) : (Q_HALFS > O_HALFS ? Q_HALFS : O_HALFS);
+    __shared__ __attribute__((aligned(16))) _Float16 smem[SMEM_HALFS];
+    __shared__ uint32_t s_list[HAS_MASK ? kTileListCap : 1];
+    __shared__ int s_wave_cnt[4];
+    __shared__ uint32_t s_qmax[kPrefillQueriesPerBlock];
+    _Float16 (*sK)[BN][LDK] = reinterpret_cast<_Float16 (*)[BN][LDK]>(smem);
+    _Float16 (*sV)[BN][LDV] = reinterpret_cast<_Float16 (*)[BN][LDV]>(smem + 2 * BN * LDK);
+
+    const Kv8Params &p = pp.k;
+    const Params &a = p.a;
+    const PrefillParams &pf = pp.f;
+    const int BH = a.B * a.H, S = p.S, P = a.start_pos, L = a.L;
+    int qb, bh;
+    prefill_block_to_tile((int)blockIdx.x, BH, (S + kPrefillQueriesPerBlock - 1) / kPrefillQueriesPerBlock, HAS_MASK, qb, bh);
+    const int ctx = P + S, ctx8 = ctx & ~(p.T - 1); // rows [0, ctx8) are bytes, [ctx8, ctx) wait in the tail
+    const int NT = (ctx + BN - 1) / BN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int qi = lane & 31, hf = lane >> 5;
+    const int q_row = qb * kPrefillQueriesPerBlock + wave * 32 + qi;
+
+    auto build_list = [&](int c0, int c1, bool have_first, uint32_t w_first) __attribute__((always_inline)) -> int {
+        return build_tile_list(pf, qb, c0, c1, NT, have_first, w_first, s_list, s_wave_cnt);
+    };
+    auto list_entry = [&](int c0, int i) __attribute__((always_inline)) -> uint32_t {
+        if constexpr (HAS_MASK) return s_list[i];
+        else return (uint32_t)(c0 + i) << 8 | 0x55u;
+    };
+
+    // global -> registers (fetch), registers -> LDS (commit) of a key tile: bytes, or fp16 rows of the tail (twice as many
+    // loads), whose rows behind the context arrive as zeros.
+    const size_t row_off = (size_t)bh * L * D, tail_off = (size_t)bh * p.T * D;
+    u32x4 stage[LPT], stage_hi[LPT]; // (stage_hi: tail rows only)
+    auto fetch = [&](int t) __attribute__((always_inline)) {
+        const bool tail = t * BN >= ctx8; // uniform
+#pragma unroll
+        for (int j = 0; j < LPT; ++j) {
+            const bool is_v = (wave + 4 * j) * 64 >= NCH; // uniform: NCH is a multiple of 64
+            const int i = tid + j * 256 - (is_v ? NCH : 0);
+            const int r = i / CPR8, e0 = (i % CPR8) * 16;
+            if (2 * NCH % 256 == 0 || (wave + 4 * j) * 64 < 2 * NCH) {
+                if (!tail) {
+                    stage[j] = *reinterpret_cast<const u32x4 *>((is_v ? p.v8 : p.k8) + row_off + (size_t)t * (BN * D) + (r * D + e0));
+                } else {
+                    const int row = t * BN + r - ctx8;
+                    const _Float16 *src = (is_v ? p.v_tail : p.k_tail) + tail_off + (size_t)min(row, ctx - ctx8 - 1) * D + e0;
+                    stage[j] = *reinterpret_cast<const u32x4 *>(src);
+                    stage_hi[j] = *reinterpret_cast<const u32x4 *>(src + 8);
+                    if (row >= ctx - ctx8) stage[j] = stage_hi[j] = u32x4{0, 0, 0, 0};
+                }
+            }
+        }
+    };
+    auto commit = [&](int t, int buf) __attribute__((always_inline)) {
+        const bool tail = t * BN >= ctx8;
+#pragma unroll
+        for (int j = 0; j < LPT; ++j) {
+            const bool is_v = (wave + 4 * j) * 64 >= NCH;
+            const int i = tid + j * 256 - (is_v ? NCH : 0);
+            const int r = i / CPR8, e0 = (i % CPR8) * 16;
+            if (2 * NCH % 256 == 0 || (wave + 4 * j) * 64 < 2 * NCH) {
+                half8 y0, y1;
+                if (!tail) {
+                    half2v h[8];
+                    widen4(stage[j][0], h[0], h[1]);
+                    widen4(stage[j][1], h[2], h[3]);
+                    widen4(stage[j][2], h[4], h[5]);
+                    widen4(stage[j][3], h[6], h[7]);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) { y0[c] = h[c / 2][c % 2]; y1[c] = h[4 + c / 2][c % 2]; }
+                } else {
+                    y0 = __builtin_bit_cast(half8, stage[j]);
+                    y1 = __builtin_bit_cast(half8, stage_hi[j]);
+                }
+                half8 *dst = reinterpret_cast<half8 *>(is_v ? &sV[buf][r][e0] : &sK[buf][r][e0]);
+                dst[0] = y0;
+                dst[1] = y1;
+            }
+        }
+    };
+
+    const int first_c1 = min(kTileListCap, NT);
+    fetch(0); // a guess at the first listed tile: right without a mask and under every causal one
+    uint32_t w_first = 0;
+    if constexpr (HAS_MASK) {
+        if (tid < first_c1) w_first = tile_class_word(pf, qb, tid, NT);
+    }
+
+    // The rotated queries as fp16 pairs in operand layout, by way of LDS: every wave its own 32 (see the fp16 caches'
+    // kernel for the data path), scaled by a power of two that comes back in qc.
+    half8 qhi[NC], qlo[NC];
+    float qc; // softmax scale * log2 e / that power, of this lane's query
+    {
+        constexpr int CPR = D / 8, QPL = 32 * CPR / 64;
+        constexpr bool FIXED_COL = 64 % CPR == 0;
+        constexpr int RPI = FIXED_COL ? 64 / CPR : 1;
+        auto q_rl = [&](int j) __attribute__((always_inline)) -> int { return FIXED_COL ? lane / CPR + j * RPI : (lane + 64 * j) / CPR; };
+        auto q_cc = [&](int j) __attribute__((always_inline)) -> int { return FIXED_COL ? lane % CPR : (lane + 64 * j) % CPR; };
+        const int b = bh / a.H, h = bh % a.H, row0 = a.rope_row < 0 ? P : a.rope_row;
+        const int q_first = qb * kPrefillQueriesPerBlock + wave * 32;
+        _Float16 *const sq = smem + wave * 32 * LDQ;
+        float x[QPL][8];
+        auto load_queries = [&](auto kind_tag) __attribute__((always_inline)) {
+            constexpr int KIND = decltype(kind_tag)::value;
+            constexpr int BATCH = KIND != kInF16 && QPL > 1 ? QPL / 2 : QPL;
+#pragma unroll
+            for (int j0 = 0; j0 < QPL; j0 += BATCH) {
+                u32x4 raw[BATCH][KIND == kInF16 ? 1 : 2];
+                float4 f[BATCH][2], w[KIND == kInI32 ? BATCH : 1][2];
+                float sc[KIND == kInI32 ? BATCH : 1];
+#pragma unroll
+                for (int jj = 0; jj < BATCH; ++jj) { // rows past the prompt read its last one and are zeroed below
+                    const int cc = q_cc(j0 + jj), q = min(q_first + q_rl(j0 + jj), S - 1);
+                    const int64_t token = (int64_t)b * S + q;
+                    const size_t off = (size_t)(token * a.H + h) * D + cc * 8;
+                    if constexpr (KIND == kInF16) {
+                        raw[jj][0] = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const _Float16 *>(a.q) + off);
+                    } else {
+                        const u32x4 *src = reinterpret_cast<const u32x4 *>(reinterpret_cast<const float *>(a.q) + off);
+                        raw[jj][0] = src[0];
+                        raw[jj][1] = src[1];
+                    }
+                    if constexpr (KIND == kInI32) {
+                        sc[jj] = a.inp_scale[token];
+                        w[jj][0] = *reinterpret_cast<const float4 *>(a.wq_scale + h * D + cc * 8);
+                        w[jj][1] = *reinterpret_cast<const float4 *>(a.wq_scale + h * D + cc * 8 + 4);
+                    }
+                    const float4 *fr = reinterpret_cast<const float4 *>(a.freq_cis + (size_t)(row0 + q) * D + cc * 8);
+                    f[jj][0] = fr[0];
+                    f[jj][1] = fr[1];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int jj = 0; jj < BATCH; ++jj) {
+                    float v[8];
+                    if constexpr (KIND == kInF16) {
+                        const half8 y = __builtin_bit_cast(half8, raw[jj][0]);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = (float)y[i];
+                    } else if constexpr (KIND == kInF32) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(raw[jj][i / 4][i % 4]);
+                    } else {
+                        const float ws[8] = {w[jj][0].x, w[jj][0].y, w[jj][0].z, w[jj][0].w, w[jj][1].x, w[jj][1].y, w[jj][1].z, w[jj][1].w};
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn((float)(int)raw[jj][i / 4][i % 4], sc[jj]), ws[i]);
+                    }
+                    const bool valid = q_first + q_rl(j0 + jj) < S;
+                    float *o = x[j0 + jj];
+                    rope_pair(v[0], v[1], f[jj][0].x, f[jj][0].y, o[0], o[1]);
+                    rope_pair(v[2], v[3], f[jj][0].z, f[jj][0].w, o[2], o[3]);
+                    rope_pair(v[4], v[5], f[jj][1].x, f[jj][1].y, o[4], o[5]);
+                    rope_pair(v[6], v[7], f[jj][1].z, f[jj][1].w, o[6], o[7]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = valid ? o[i] : 0.f;
+                }
+            }
+        };
+        if (p.in_kind == kInF16) load_queries(std::integral_constant<int, kInF16>{});
+        else if (p.in_kind == kInF32) load_queries(std::integral_constant<int, kInF32>{});
+        else load_queries(std::integral_constant<int, kInI32>{});
+
+        // largest |element| of every query (bit patterns of non-negative floats order as integers)
+        uint32_t *const qmax = s_qmax + wave * 32;
+        if (lane < 32) qmax[lane] = 0u;
+        wave_lds_sync();
+#pragma unroll
+        for (int j = 0; j < QPL; ++j) {
+            float top = 1e-30f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[j][i]));
+            if constexpr (FIXED_COL) {
+                top = fmaxf(top, dpp_move<0xB1>(top));
+                top = fmaxf(top, dpp_move<0x4E>(top));
+                if constexpr (CPR >= 8) top = fmaxf(top, dpp_move<0x141>(top));
+                if constexpr (CPR >= 16) top = fmaxf(top, dpp_move<0x140>(top));
+                if (lane % CPR == 0) qmax[q_rl(j)] = __float_as_uint(top);
+            } else {
+                atomicMax(&qmax[q_rl(j)], __float_as_uint(top));
+            }
+        }
+        wave_lds_sync();
+        auto power = [&](uint32_t top_bits) __attribute__((always_inline)) -> float { // 2^(8 - floor(log2 top))
+            return __uint_as_float((uint32_t)(127 + 8 + 127 - (int)(top_bits >> 23)) << 23);
+        };
+        half8 lo_keep[QPL];
+#pragma unroll
+        for (int j = 0; j < QPL; ++j) {
+            const float f = power(qmax[q_rl(j)]);
+            half8 hq;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = x[j][i] * f;
+                hq[i] = (_Float16)y;
+                lo_keep[j][i] = (_Float16)(y - (float)hq[i]);
+            }
+            *reinterpret_cast<half8 *>(sq + q_rl(j) * LDQ + q_cc(j) * 8) = hq;
+        }
+        wave_lds_sync();
+#pragma unroll
+        for (int c = 0; c < NC; ++c) qhi[c] = *reinterpret_cast<const half8 *>(sq + qi * LDQ + 16 * c + 8 * hf);
+        wave_lds_sync();
+#pragma unroll
+        for (int j = 0; j < QPL; ++j) *reinterpret_cast<half8 *>(sq + q_rl(j) * LDQ + q_cc(j) * 8) = lo_keep[j];
+        wave_lds_sync();
+#pragma unroll
+        for (int c = 0; c < NC; ++c) qlo[c] = *reinterpret_cast<const half8 *>(sq + qi * LDQ + 16 * c + 8 * hf);
+        const uint32_t e = qmax[qi] >> 23; // biased exponent of the largest element
+        qc = a.scale * kLog2e * __uint_as_float((uint32_t)((int)e - 8) << 23);
+        const int block = q_first / 32 - pp.first_block;
+        if (pp.q_pairs && block >= 0 && q_first < S) { // kept for the block weights
+            half8 *dst = pp.q_pairs + ((size_t)bh * pp.kept_blocks + block) * (2 * NC * 64) + lane;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                dst[c * 64] = qhi[c];
+                dst[(NC + c) * 64] = qlo[c];
+            }
+            if (hf == 0) pp.q_factor[((size_t)bh * pp.kept_blocks + block) * 32 + qi] = qc;
+        }
+    }
+    if constexpr (!HAS_MASK) __syncthreads(); // the slices lie in the tile buffers (with a mask the list's barriers see to it)
+    int n_first = first_c1;
+    if constexpr (HAS_MASK) n_first = build_list(0, first_c1, true, w_first);
+    if (n_first > 0) {
+        const int t_first = (int)(__builtin_amdgcn_readfirstlane(list_entry(0, 0)) >> 8);
+        if (t_first != 0) fetch(t_first);
+    }
+
+    floatx16 ot[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) ot[dt][v] = 0.f;
+    float m = kMaxFloor * kLog2e, l = 0.f;
+    uint32_t vref = 0u; // bits of the power of two that the output accumulators are in units of (uniform); 0: none yet
+    const int vrow = 4 * hf + ((lane & 15) >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const float *ks_at = p.k_scale + (size_t)bh * p.nblk, *vs_at = p.v_scale + (size_t)bh * p.nblk;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) asm volatile("" : "+v"(qhi[c]), "+v"(qlo[c]));
+
+    for (int c0 = 0; c0 < NT; c0 += kTileListCap) {
+        const int c1 = min(c0 + kTileListCap, NT);
+        int n = c1 - c0;
+        if (c0 == 0) n = n_first;
+        else if constexpr (HAS_MASK) n = build_list(c0, c1, false, 0u); // ends with a barrier
+        else __syncthreads();
+        if (n == 0) continue;
+        uint32_t e0 = __builtin_amdgcn_readfirstlane(list_entry(c0, 0));
+        uint32_t e1 = n > 1 ? __builtin_amdgcn_readfirstlane(list_entry(c0, 1)) : 0u;
+        uint32_t e2 = n > 2 ? __builtin_amdgcn_readfirstlane(list_entry(c0, 2)) : 0u;
+        if (c0 > 0) fetch((int)(e0 >> 8));
+        commit((int)(e0 >> 8), 0);
+        if (n > 1) fetch((int)(e1 >> 8));
+        auto tile_step = [&](int i, auto buf_tag) __attribute__((always_inline)) {
+            constexpr int buf = decltype(buf_tag)::value;
+            const int t = (int)(e0 >> 8), k0 = t * BN;
+            float ks = 1.f, vs = 1.f; // tail rows are values themselves
+            if (k0 < ctx8) {
+                ks = ks_at[k0 >> p.t_shift];
+                vs = vs_at[k0 >> p.t_shift];
+            }
+            __syncthreads(); // tile t is visible; every wave is done with the other buffer
+            uint32_t tc = kTileZero;
+            if constexpr (HAS_MASK) tc = __builtin_amdgcn_readfirstlane((e0 >> (2 * wave)) & 3u);
+            const bool special = tc != kTileSkip && (k0 + BN > ctx || tc >= kTileMixed);
+            float mk[16];
+            if constexpr (HAS_MASK) {
+                if (special && tc == kTileMixed) { // before the next tile is requested: loads return in order
+                    const float *mrow = pf.attn_mask + (size_t)(P + min(q_row, S - 1)) * pf.mask_ld;
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) mk[v] = mrow[min(k0 + 8 * (v / 4) + 4 * hf + (v % 4), ctx - 1)];
+                }
+            }
+            if (i + 1 < n) {
+                commit((int)(e1 >> 8), buf ^ 1);
+                if (i + 2 < n) fetch((int)(e2 >> 8));
+            }
+            if (tc != kTileSkip) {
+                floatx16 st;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) st[v] = 0.f;
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const half8 ka = *reinterpret_cast<const half8 *>(&sK[buf][qi][16 * c + 8 * hf]);
+                    st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qlo[c], st, 0, 0, 0);
+                    st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qhi[c], st, 0, 0, 0);
+                }
+                float cs = qc * ks; // raw product -> base-2 score
+                if (special) {
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) {
+                        const int key = 8 * (v / 4) + 4 * hf + (v % 4);
+                        float s = st[v] * cs;
+                        if constexpr (HAS_MASK) {
+                            if (tc == kTileMixed) s = fmaf(mk[v], kLog2e, s);
+                            if (tc == kTileDiag && key > qi) s = -__builtin_inff();
+                        }
+                        st[v] = k0 + key >= ctx ? -__builtin_inff() : s;
+                    }
+                    cs = 1.f;
+                }
+                // The accumulators' unit: a power of two no smaller than any block's scale so far.
+                if (vs == 0.f) vs = 1.f; // a block of zeros
+                const uint32_t vbits = __builtin_amdgcn_readfirstlane((__float_as_uint(vs) + 0x7fffffu) & 0xff800000u);
+                if (vbits > vref) { // uniform
+                    const float down = __uint_as_float(vref) / __uint_as_float(vbits);
+                    vref = vbits;
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) ot[dt][v] *= down;
+                }
+                const float lr = __builtin_amdgcn_logf(vs / __uint_as_float(vref)) + kKv8WeightExp; // log2
+                const float mx = fmaxf(m, cross_half_max(max16(st)) * cs);
+                if (__ballot(mx > m + kLazyMax) != 0ull) { // wave-uniform
+                    const float alpha = __builtin_amdgcn_exp2f(m - mx);
+                    m = mx;
+                    l *= alpha;
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) ot[dt][v] *= alpha;
+                }
+                const float nb = lr - m;
+                half8 ph[2], pl[2];
+                float sum = 0.f;
+#pragma unroll
+                for (int v = 0; v < 16; v += 2) {
+                    float2v e;
+                    e[0] = __builtin_amdgcn_exp2f(fmaf(st[v], cs, nb));
+                    e[1] = __builtin_amdgcn_exp2f(fmaf(st[v + 1], cs, nb));
+                    sum += e[0];
+                    sum += e[1];
+                    const half2v h = __builtin_convertvector(e, half2v);
+                    ph[v / 8][v % 8] = h[0];
+                    ph[v / 8][v % 8 + 1] = h[1];
+                    pl[v / 8][v % 8] = (_Float16)fmaf(-(float)h[0], 1.0f, e[0]);
+                    pl[v / 8][v % 8 + 1] = (_Float16)fmaf(-(float)h[1], 1.0f, e[1]);
+                }
+                l = fmaf(sum, __builtin_amdgcn_exp2f(-lr), l);
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const half4 lo = lds_read_tr16(&sV[buf][16 * u + vrow][32 * dt + vcol]);
+                        const half4 hi = lds_read_tr16(&sV[buf][16 * u + 8 + vrow][32 * dt + vcol]);
+                        half8 va;
+                        va[0] = lo[0]; va[1] = lo[1]; va[2] = lo[2]; va[3] = lo[3];
+                        va[4] = hi[0]; va[5] = hi[1]; va[6] = hi[2]; va[7] = hi[3];
+                        ot[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[u], ot[dt], 0, 0, 0);
+                        ot[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], ot[dt], 0, 0, 0);
+                    }
+                }
+            }
+            e0 = e1;
+            e1 = e2;
+            e2 = i + 3 < n ? __builtin_amdgcn_readfirstlane(list_entry(c0, i + 3)) : 0u;
+        };
+        for (int i = 0; i < n; i += 2) {
+            tile_step(i, std::integral_constant<int, 0>{});
+            if (i + 1 < n) tile_step(i + 1, std::integral_constant<int, 1>{});
+        }
+    }
+
+    l += __shfl_xor(l, 32);
+    if (p.stats && hf == 0 && q_row < S) p.stats[(size_t)bh * S + q_row] = make_float2(m, l);
+    // e^(..) sums to l, accumulators are in units of vref with weights times 2^7; a fully masked query: 0 / 0
+    const float rl = __uint_as_float(vref) * (1.0f / 128.0f) / l;
+    __syncthreads(); // every wave is done with the last tile
+    float *so = reinterpret_cast<float *>(smem) + wave * 32 * LDO;
+    const int q0 = qb * kPrefillQueriesPerBlock + wave * 32;
+    float *dst0 = a.out + ((size_t)bh * S + q0) * D;
+    constexpr int LPRW = HALF_D / 4, ROWS = 64 / LPRW;
+#pragma unroll
+    for (int pass = 0; pass < D / HALF_D; ++pass) {
+#pragma unroll
+        for (int dd = 0; dd < HALF_D / 32; ++dd) {
+            const int dt = pass * (HALF_D / 32) + dd;
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4)
+                *reinterpret_cast<float4 *>(so + qi * LDO + 32 * dd + 8 * g4 + 4 * hf) =
+                    make_float4(ot[dt][4 * g4 + 0] * rl, ot[dt][4 * g4 + 1] * rl, ot[dt][4 * g4 + 2] * rl, ot[dt][4 * g4 + 3] * rl);
+        }
+        wave_lds_sync();
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += ROWS) {
+            const int r = r0 + lane / LPRW, c4 = lane % LPRW;
+            const float4 v = *reinterpret_cast<const float4 *>(so + r * LDO + 4 * c4);
+            if (q0 + r < S) *reinterpret_cast<float4 *>(dst0 + (size_t)r * D + pass * HALF_D + 4 * c4) = v;
+        }
+        wave_lds_sync(); // the slice is rewritten by the next pass
+    }
+}
+
+// Block weights of a prompt: weights[b,h,blk] (+)= sum over the last weight_queries queries and the block's rows of
+// 2^(s' - m') / l, with the operands and statistics the attention kernel left.  grid = blocks * B*H, block = 256.  A wave keeps
+// 32 keys of the block in registers as operands and takes every (128 / T)-th 32-query block; the sum is formed in one order,
+// so it is the same from run to run.
+template <int D, int T>
+__global__ __launch_bounds__(256) void kv8_prompt_weights_kernel(const Kv8PromptParams pp)
+{
+    constexpr int NC = D / 16, NTB = T / 32, NQ = 4 / NTB; // key tiles of a block, waves that share a key tile
+    __shared__ float s_sum[4];
+    const Kv8Params &p = pp.k;
+    const Params &a = p.a;
+    const int S = p.S, P = a.start_pos, ctx = P + S, NT = (ctx + 31) / 32;
+    const int nb = (ctx + T - 1) / T;
+    const int blk = blockIdx.x % nb, bh = blockIdx.x / nb;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 31, hf = lane >> 5;
+    const int k0 = blk * T + 32 * (wave / NQ); // this wave's first key
+    const bool open = blk * T + T > ctx;
+    const float ks = open ? 1.f : p.k_scale[(size_t)bh * p.nblk + blk];
+    half8 ka[NC]; // key k0 + qi, elements 16c + 8hf ..
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        if (open) {
+            half8 z = half8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (k0 + qi < ctx) z = *reinterpret_cast<const half8 *>(p.k_tail + ((size_t)bh * T + (k0 + qi - blk * T)) * D + 16 * c + 8 * hf);
+            ka[c] = z;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2 *>(p.k8 + ((size_t)bh * a.L + k0 + qi) * D + 16 * c + 8 * hf);
+            half2v h[4];
+            widen4(x.x, h[0], h[1]);
+            widen4(x.y, h[2], h[3]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ka[c][i] = h[i / 2][i % 2];
+        }
+    }
+    const int first_query = S - p.weight_queries;
+    float sum = 0.f;
+    for (int block = k0 < ctx ? wave % NQ : pp.kept_blocks; block < pp.kept_blocks; block += NQ) {
+        const int q0 = (pp.first_block + block) * 32;
+        uint32_t cls = kTileZero;
+        if (a.attn_mask) cls = (tile_class_word(pp.f, q0 / kPrefillQueriesPerBlock, k0 / 32, NT) >> (8 * (q0 / 32 % 4))) & 0xffu;
+        cls = __builtin_amdgcn_readfirstlane(cls);
+        if (cls == kTileSkip) continue;
+        const size_t kept = (size_t)bh * pp.kept_blocks + block;
+        const half8 *src = pp.q_pairs + kept * (2 * NC * 64) + lane;
+        half8 qhi[NC], qlo[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            qhi[c] = src[c * 64];
+            qlo[c] = src[(NC + c) * 64];
+        }
+        const int q = q0 + qi, q_in = min(q, S - 1);
+        const float2 ml = p.stats[(size_t)bh * S + q_in];
+        const float cs = pp.q_factor[kept * 32 + qi] * ks;
+        floatx16 st;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) st[v] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[c], qlo[c], st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[c], qhi[c], st, 0, 0, 0);
+        }
+        if (cls >= kTileMixed || k0 + 32 > ctx) { // uniform
+            const float *mrow = a.attn_mask + (size_t)(P + q_in) * a.mask_ld;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int key = 8 * (v / 4) + 4 * hf + (v % 4);
+                float x = st[v] * cs;
+                if (cls == kTileMixed) x = fmaf(mrow[min(k0 + key, ctx - 1)], kLog2e, x);
+                st[v] = (cls == kTileDiag && key > qi) || k0 + key >= ctx ? -__builtin_inff() : x - ml.x;
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) st[v] = fmaf(st[v], cs, -ml.x);
+        }
+        float part = 0.f;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) part += __builtin_amdgcn_exp2f(st[v]);
+        // a query of the call that counts, and that saw a key
+        if (q >= first_query && q < S && ml.y > 0.f) sum += part / ml.y;
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        const float w = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        float *dst = p.weights + (size_t)bh * p.nblk + blk;
+        *dst = blk * T >= P ? w : *dst + w;
+    }
+}
+
+} // namespace flattn
