@@ -49,37 +49,33 @@ int granule_rows(int D) // Kv8Geometry<D>::GR
     return wt < 32 ? wt : 32;
 }
 
-// ---- launch planning of the decode step: context splits, whole multiples of kChunkRows each
+// ---- launch planning of the decode step: `nsplit` workgroups per (b,h), all but the last with a multiple of kChunkRows rows of
+// the complete blocks, the last with the open block (its rows are few, but the append comes first); a context that is
+// not split is one workgroup.
 constexpr size_t kRaggedChunkBytes = 256 * 1024;
 
-int uniform_splits(const fl_attn_desc *d, int ctx)
+int byte_splits(const fl_attn_desc *d, int ctx, bool ragged)
 {
     const int64_t bh = (int64_t)d->batch_size * d->head_num;
     int64_t n = (device_cus() + bh - 1) / bh;
-    const int64_t most = ((int64_t)ctx + kChunkRows - 1) / kChunkRows;
-    if (n > most) n = most;
     if (ctx <= 2 * kChunkRows) n = 1;
-    return (int)(n < 1 ? 1 : (n > kMaxSplits ? kMaxSplits : n));
-}
-
-int ragged_splits(const fl_attn_desc *d, int ctx)
-{
-    int64_t n = uniform_splits(d, ctx);
-    const int64_t by_bytes = ((int64_t)ctx * 2 * d->size_per_head + kRaggedChunkBytes - 1) / (int64_t)kRaggedChunkBytes;
+    if (ragged) { // work per (b,h) varies
+        const int64_t by_bytes = ((int64_t)ctx * 2 * d->size_per_head + kRaggedChunkBytes - 1) / (int64_t)kRaggedChunkBytes;
+        if (by_bytes > n) n = by_bytes;
+    }
+    if (d->nsplit > 0) n = d->nsplit;
     const int64_t most = ((int64_t)ctx + kChunkRows - 1) / kChunkRows;
-    if (by_bytes > n) n = by_bytes;
     if (n > most) n = most;
-    return (int)(n < 1 ? 1 : (n > kMaxSplits ? kMaxSplits : n));
+    return (int)(n < 1 ? 1 : (n > kMaxSplits - 1 ? kMaxSplits - 1 : n));
 }
 
-int split_cap(const fl_attn_desc *d) { return d->nsplit > 0 ? d->nsplit : ragged_splits(d, d->total_len); }
+int split_cap(const fl_attn_desc *d) { return byte_splits(d, d->total_len, true) + 1; }
 
 void make_plan(const fl_attn_desc *d, int ctx, bool ragged, fl_attn_plan *plan)
 {
-    const int n = d->nsplit > 0 ? d->nsplit : (ragged ? ragged_splits(d, ctx) : uniform_splits(d, ctx));
-    const int chunk = ((ctx + n - 1) / n + kChunkRows - 1) / kChunkRows * kChunkRows;
-    plan->chunk_rows = chunk;
-    plan->nsplit = (ctx + chunk - 1) / chunk;
+    const int n = byte_splits(d, ctx, ragged);
+    plan->chunk_rows = ((ctx + n - 1) / n + kChunkRows - 1) / kChunkRows * kChunkRows;
+    plan->nsplit = n == 1 ? 1 : (ctx + plan->chunk_rows - 1) / plan->chunk_rows + 1;
     plan->threads = flattn::kKv8Waves * 64;
     plan->two_pass = plan->nsplit <= 1 ? 0 : ((int64_t)plan->nsplit * d->batch_size * d->head_num <= 4 * (int64_t)device_cus() ? 2 : 1);
 }

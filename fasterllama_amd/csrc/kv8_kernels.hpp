@@ -74,7 +74,45 @@ __device__ __forceinline__ void load_input(const void *base, int kind, size_t of
     }
 }
 
-// RoPE of N consecutive elements by their table entries.
+// The same in two steps for 16 elements, so that other loads can be issued between: raw words, then values.
+struct RawInput { u32x4 w[4]; };
+__device__ __forceinline__ void request_input(const void *base, int kind, size_t off, RawInput &raw)
+{
+    const u32x4 *src = kind == kInF16 ? reinterpret_cast<const u32x4 *>(reinterpret_cast<const _Float16 *>(base) + off)
+                                      : reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint32_t *>(base) + off);
+    raw.w[0] = src[0];
+    raw.w[1] = src[1];
+    if (kind != kInF16) {
+        raw.w[2] = src[2];
+        raw.w[3] = src[3];
+    }
+}
+__device__ __forceinline__ void input_values(const RawInput &raw, int kind, float inp_scale, const float *w_scale_at, float (&dst)[16])
+{
+    if (kind == kInF16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dst[i] = (float)__builtin_bit_cast(half8, raw.w[i / 8])[i % 8];
+    } else if (kind == kInF32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dst[i] = __uint_as_float(raw.w[i / 4][i % 4]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dst[i] = __fmul_rn(__fmul_rn((float)(int)raw.w[i / 4][i % 4], inp_scale), w_scale_at[i]);
+    }
+}
+
+// RoPE of 16 consecutive elements by their table entries, from registers or from memory.
+__device__ __forceinline__ void rotate_by(float (&x)[16], const float4 (&f)[4])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float r0, r1, r2, r3;
+        rope_pair(x[4 * i], x[4 * i + 1], f[i].x, f[i].y, r0, r1);
+        rope_pair(x[4 * i + 2], x[4 * i + 3], f[i].z, f[i].w, r2, r3);
+        x[4 * i] = r0; x[4 * i + 1] = r1; x[4 * i + 2] = r2; x[4 * i + 3] = r3;
+    }
+}
+
 template <int N>
 __device__ __forceinline__ void rotate_run(float (&x)[N], const float *freq_at)
 {
@@ -162,7 +200,8 @@ struct Kv8Geometry {
     static constexpr int U = 4;                     // load instructions per matrix in flight
     static constexpr int WT = GPW * U;              // rows per wave and trip
     static constexpr int GR = WT < 32 ? WT : 32;    // rows per granule of the weight sums
-    static constexpr int NS = WT > 32 ? WT / 32 : 1; // 32-row groups per trip: each has one scale
+    static constexpr int NG = WT / GR;              // granules per trip: each has one scale
+    static constexpr int BATCH = 64 / NG;           // trips whose granules fill the lanes of a wave
 };
 
 constexpr float kKv8LazyMax = 8.0f; // base-2 units: the running reference maximum may lag the true one by this much
@@ -170,30 +209,35 @@ constexpr float kQDigits = 8300000.0f; // |q| maps to at most this: three balanc
 constexpr int kKv8Waves = 4;
 
 // Adds the softmax weight of every block to weights[b,h,:], from the granules and the merged statistics (M, Lsum) of the
-// row.  A block whose first row arrived in this step starts from 0.
-template <int D>
-__device__ __forceinline__ void add_block_weights(const Kv8Params &p, int bh, int P, float M, float Lsum, int tid)
+// row.  A block whose first row arrived in this step starts from 0.  old: this thread's first block's weight so far.
+template <int D, typename LOAD>
+__device__ __forceinline__ void add_block_weights(const Kv8Params &p, int bh, int P, float M, float Lsum, int tid, LOAD granule, float old)
 {
     constexpr int GR = Kv8Geometry<D>::GR;
     if (!(Lsum > 0.f)) return; // every key masked: the output is NaN, nothing was attended to
     const int blk_new = P >> p.t_shift;
     const bool open = ((P + 1) & (p.T - 1)) != 0; // the last block's rows are in the tail: one granule for all of them
-    const float2 *g = p.granules + (size_t)bh * (p.a.L / GR);
     const int per = p.T / GR;
     const float rl = 1.0f / Lsum;
     for (int blk = tid; blk <= blk_new; blk += kKv8Waves * 64) {
         float w = 0.f;
         const int n = open && blk == blk_new ? 1 : per;
         for (int i = 0; i < n; ++i) {
-            const float *e = reinterpret_cast<const float *>(g + (size_t)blk * per + i);
-            const float m = load_partial<true>(e), s = load_partial<true>(e + 1);
-            w = fmaf(s, __builtin_amdgcn_exp2f(m - M), w);
+            const float2 ms = granule(blk * per + i);
+            w = fmaf(ms.y, __builtin_amdgcn_exp2f(ms.x - M), w);
         }
         float *dst = p.weights + (size_t)bh * p.nblk + blk;
         const bool fresh = blk == blk_new && (P & (p.T - 1)) == 0;
-        *dst = fresh ? w * rl : fmaf(w, rl, *dst);
+        *dst = fresh ? w * rl : fmaf(w, rl, blk == tid ? old : *dst);
     }
 }
+
+// Granules that other workgroups, or other waves through memory, have written.
+struct GranuleLoader {
+    const float *at;
+    __device__ __forceinline__ float2 operator()(int i) const { return make_float2(load_partial<true>(at + 2 * i), load_partial<true>(at + 2 * i + 1)); }
+};
+__device__ __forceinline__ GranuleLoader granule_loader(const float2 *at) { return GranuleLoader{reinterpret_cast<const float *>(at)}; }
 
 // Quantises one full tail (T rows of one (b,h)) into block `blk`, by the 256 threads of a workgroup.  Two passes over
 // the tail: T * D halfs, which the second finds in the caches.
@@ -224,25 +268,36 @@ __device__ __forceinline__ void quantise_tail(const _Float16 *tail, int8_t *rows
     if (tid == 0) *scale_at = absmax / 127.0f;
 }
 
+// Splits of one (b,h) in a decode step whose context is split: `chunk` rows of the complete blocks each, and one more for the
+// newest row and the open block's rows before it (or for the block that the newest row completes).
+__device__ __forceinline__ int kv8_splits(const Params &a, int T, int P) { return (P - (P & (T - 1)) + a.chunk - 1) / a.chunk + 1; }
+
 // One decode step (PROMPT = false): grid = splits * B * H workgroups of four waves, (b,h) fastest as in the streaming
-// kernel of the other cache types; a workgroup streams `chunk` rows (a multiple of 128) of one (b,h), four rows per lane
-// group and trip.  PROMPT = true: one workgroup per (b, query, h) over the rows as they are, no append — the prompt phase
-// of the head sizes the matrix-core kernel does not serve.
+// kernel of the other cache types.  PROMPT = true: one workgroup per (b, query, h) over the rows as they are, no append — the
+// prompt phase of the head sizes the matrix-core kernel does not serve.
 //
-// A row of D bytes is D/16 lanes.  Scores: the query enters as integers of three base-256 digits, q = qs * (d0 + 256 d1 +
-// 65536 d2) with |error| <= 2^-24 of its largest element, so K needs no conversion: twelve v_dot4_i32_i8 per 16 bytes
-// multiply the bytes as they come (exactly), against 32 instructions for conversion and FMA.  V bytes are converted (one
-// instruction each) and accumulated in FP32.  The running maximum is shared by the whole wave, which makes the weights of
-// different rows comparable at once (granule sums) and the rescale of the accumulators a rare, wave-uniform branch.
+// A row of D bytes is D/16 lanes; a wave takes four load instructions of K and four of V per trip.  Scores: the query enters
+// as integers of three base-256 digits, q = qs * (d0 + 256 d1 + 65536 d2) with |error| <= 2^-24 of its largest element, so K
+// needs no conversion: twelve v_dot4_i32_i8 per 16 bytes multiply the bytes as they come (exactly), against 32 instructions
+// for conversion and FMA.  V bytes are converted (one instruction each) and accumulated in FP32.  The running maximum is
+// shared by the whole wave, which makes the weights of different rows comparable at once (granule sums) and the rescale of
+// the accumulators a rare, wave-uniform branch.
+//
+// Bound by HBM at large batches: the loads never stop.  K of the next trip is requested into K's registers as soon as the
+// scores are formed, V's as soon as V is used up, so either half of a trip's arithmetic has the other matrix's loads in
+// flight, at no register's cost; the first trip is requested before the query has arrived.
 template <int D, bool HAS_MASK, bool PROMPT>
-__global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Params p)
+__global__ __launch_bounds__(kKv8Waves * 64) __attribute__((amdgpu_waves_per_eu(3, 8)))
+void kv8_attn_kernel(const Kv8Params p)
 {
     typedef Kv8Geometry<D> G;
     constexpr int LPR = G::LPR, GPW = G::GPW, U = G::U, WT = G::WT, GR = G::GR;
+    constexpr bool CHECK = WT > 32; // a trip may reach over the end of the rows (blocks are multiples of 32)
     static_assert(kKv8Waves * 64 == kCombineThreads, "the merge runs on a 256-thread workgroup");
     __shared__ float s_o[kKv8Waves][D];
     __shared__ float s_m[kKv8Waves], s_l[kKv8Waves], s_t[kKv8Waves], s_red[kKv8Waves];
-    __shared__ CombineShared<D> s_merge;
+    __shared__ __attribute__((aligned(16))) char s_merge_bytes[PROMPT ? 16 : sizeof(CombineShared<D>)];
+    constexpr int LDS_GRANULES = (int)sizeof(s_merge_bytes) / 8; // where one workgroup has all rows and does not merge
     __shared__ int s_last;
 
     const Params &a = p.a;
@@ -270,37 +325,127 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
             return;
         }
     }
-    const int ctx = P + 1;
-    const int start = PROMPT ? 0 : split * a.chunk;
-    if (start >= ctx) return;
-    const int end = PROMPT ? ctx : min(start + a.chunk, ctx);
-    const bool owner = end == ctx;                     // this workgroup has the newest row
-    const int P0 = P & ~(T - 1);
+    const bool direct = PROMPT || a.direct;
+    const int ctx = P + 1, P0 = P & ~(T - 1);
     const bool fills = ctx == P0 + T;                  // the newest row is the last of its block
-    const int end8 = owner && !fills ? P0 : end;       // rows [start, end8) come as bytes; multiples of T
+    const int splits = direct ? 1 : kv8_splits(a, T, P);
+    if (split >= splits) return;
+    const bool owner = split == splits - 1;            // this workgroup has the newest row and the open block
+    const int start = direct ? 0 : (owner ? P0 : split * a.chunk);
+    const int end8 = owner ? (fills ? ctx : P0) : min(start + a.chunk, P0); // rows [start, end8) come as bytes: whole blocks
     const int q_pos = PROMPT ? a.start_pos + s_query : P;
     const size_t row_off = (size_t)bh * L * D, tail_off = (size_t)bh * T * D;
     const bool has_chunk = !G::PADDED || lig < G::CH;
-    const int e0 = lig * 16;
+    const int e0 = lig * 16, e0_in = has_chunk ? e0 : 0; // (lanes without a chunk load the first one and drop it)
 
-    const float inp_scale = p.in_kind == kInI32 ? a.inp_scale[PROMPT ? b * p.S + s_query : b] : 0.f;
+    const int kind = p.in_kind;
+    const float inp_scale = kind == kInI32 ? a.inp_scale[PROMPT ? b * p.S + s_query : b] : 0.f;
     int rope_row = PROMPT ? (a.rope_row < 0 ? q_pos : a.rope_row + s_query) : (a.rope_row < 0 ? P : a.rope_row);
     if (!PROMPT && p.rope_rows) rope_row = p.rope_rows[b];
-    const float *freq = a.freq_cis + (size_t)rope_row * D + e0;
-    const size_t in_off = PROMPT ? ((size_t)(b * p.S + s_query) * H + h) * D + e0 : (size_t)bh * D + e0;
+    const float *freq = a.freq_cis + (size_t)rope_row * D + e0_in;
+    const size_t in_off = PROMPT ? ((size_t)(b * p.S + s_query) * H + h) * D + e0_in : (size_t)bh * D + e0_in;
+
+    // What a trip needs, in two halves.  A lane behind the last row reads nothing and receives zeros.
+    const __amdgpu_buffer_rsrc_t Kbuf = make_buffer(p.k8 + row_off), Vbuf = make_buffer(p.v8 + row_off);
+    const float *mrow = HAS_MASK ? a.attn_mask + (size_t)q_pos * a.mask_ld : nullptr;
+    const __amdgpu_buffer_rsrc_t Mbuf = make_buffer(HAS_MASK ? (const void *)mrow : (const void *)p.k8);
+    const float *ks_at = p.k_scale + (size_t)bh * p.nblk, *vs_at = p.v_scale + (size_t)bh * p.nblk;
+    const uint32_t lane_off = has_chunk ? (uint32_t)(g * D + e0) : kLaneOutOfRange;
+    u32x4 kv[U], vv[U];
+    // Mask entries: a lane fetches that of row u = lane % 4 of its group, and a quad broadcast hands entry u to every lane (one
+    // load and one register for the trip); rows of two lanes fetch one by one.
+    constexpr bool MASK_QUAD = LPR >= 4;
+    float mk[MASK_QUAD ? 1 : U];
+    const uint32_t mask_lane = (uint32_t)((MASK_QUAD ? (lane & 3) * GPW : 0) + g);
+    auto request_k = [&](int r) __attribute__((always_inline)) {
+        if constexpr (HAS_MASK) {
+#pragma unroll
+            for (int u = 0; u < (MASK_QUAD ? 1 : U); ++u) {
+                const bool in = r + u * GPW + (int)mask_lane < end8;
+                mk[u] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(Mbuf, in ? mask_lane * 4u : kLaneOutOfRange, (uint32_t)(r + u * GPW) * 4u, 0));
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = r + (CHECK ? u * GPW : 0) < end8; // uniform
+            kv[u] = __builtin_amdgcn_raw_buffer_load_b128(Kbuf, in ? lane_off : kLaneOutOfRange, (uint32_t)(r + u * GPW) * (uint32_t)D, kLoadNonTemporal);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto request_v = [&](int r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = r + (CHECK ? u * GPW : 0) < end8;
+            vv[u] = __builtin_amdgcn_raw_buffer_load_b128(Vbuf, in ? lane_off : kLaneOutOfRange, (uint32_t)(r + u * GPW) * (uint32_t)D, kLoadNonTemporal);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    int r = start + wave * WT;
+    // Scales: lane i holds those of granule i of the next BATCH trips, one load for all of them, and the trip that needs them
+    // reads that lane.  (A block that was never written may have any scale: rows behind the last take 0.)
+    float ks_lanes, vs_lanes;
+    auto lane_row = [&](int base) __attribute__((always_inline)) -> int { return base + lane / G::NG * (kKv8Waves * WT) + lane % G::NG * GR; };
+    auto request_scales = [&](int base) __attribute__((always_inline)) {
+        const int row = lane_row(base), blk = min(row >> p.t_shift, p.nblk - 1);
+        ks_lanes = row < end8 ? ks_at[blk] : 0.f;
+        vs_lanes = row < end8 ? vs_at[blk] : 0.f;
+    };
+
+    // Everything whose address is known is requested before anything is waited for: the query, the new row, the first two tail
+    // rows of every lane group, then the first trip of the byte rows.
+    const bool appends = !PROMPT && owner, has_tail = owner && !fills;
+    const bool gather = !PROMPT && p.weights != nullptr;
+    RawInput q_raw, k_raw, v_raw;
+    request_input(a.q, kind, in_off, q_raw);
+    float4 fr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fr[i] = reinterpret_cast<const float4 *>(freq)[i];
+    if (appends && wave == 0) {
+        request_input(a.k_new, kind, in_off, k_raw);
+        request_input(a.v_new, kind, in_off, v_raw);
+    }
+    constexpr int UT = 2; // tail rows per lane group and trip
+    const int n_tail = PROMPT ? ctx - P0 : P - P0; // rows to be read: the newest comes from registers
+    half8 kx[UT][2], vx[UT][2];
+    float mt[UT];
+    auto request_tail = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < UT; ++u) {
+            const int at = min(r0 + u * GPW + g, n_tail - 1);
+            const half8 *kt = reinterpret_cast<const half8 *>(p.k_tail + tail_off + e0_in + (size_t)at * D);
+            const half8 *vt = reinterpret_cast<const half8 *>(p.v_tail + tail_off + e0_in + (size_t)at * D);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                kx[u][c] = __builtin_nontemporal_load(kt + c);
+                vx[u][c] = __builtin_nontemporal_load(vt + c);
+            }
+            mt[u] = HAS_MASK ? mrow[P0 + at] : 0.f;
+        }
+    };
+    if (has_tail && wave * GPW * UT < n_tail) request_tail(wave * GPW * UT);
+    float mask_new = 0.f;
+    if (HAS_MASK && appends) mask_new = mrow[P] * kLog2e;
+    float old_weight = 0.f; // of block tid
+    if (gather && direct && tid <= P >> p.t_shift) old_weight = p.weights[(size_t)bh * p.nblk + tid];
+    __builtin_amdgcn_sched_barrier(0);
+    if (!(appends && fills)) {
+        request_scales(r);
+        request_k(r);
+        request_v(r);
+    }
 
     // The append: the new row goes to the tail; where it completes the block, the workgroup quantises the tail, and
     // the loop below finds those rows as bytes.
     half8 kn[2], vn[2];
-    if (!PROMPT && owner) {
-        if (wave == 0 && has_chunk) {
+    if (appends) {
+        if (wave == 0) {
             float x[16], y[16];
-            load_input<16>(a.k_new, p.in_kind, in_off, inp_scale, p.in_kind == kInI32 ? a.wk_scale + h * D + e0 : nullptr, x);
-            load_input<16>(a.v_new, p.in_kind, in_off, inp_scale, p.in_kind == kInI32 ? a.wv_scale + h * D + e0 : nullptr, y);
-            rotate_run<16>(x, freq);
+            input_values(k_raw, kind, inp_scale, kind == kInI32 ? a.wk_scale + h * D + e0_in : nullptr, x);
+            input_values(v_raw, kind, inp_scale, kind == kInI32 ? a.wv_scale + h * D + e0_in : nullptr, y);
+            rotate_by(x, fr);
 #pragma unroll
             for (int i = 0; i < 16; ++i) { kn[i / 8][i % 8] = stored_half(x[i]); vn[i / 8][i % 8] = stored_half(y[i]); }
-            if (g == 0) {
+            if (g == 0 && has_chunk) {
                 const size_t at = tail_off + (size_t)(P - P0) * D + e0;
                 half8 *kd = reinterpret_cast<half8 *>(p.k_tail + at), *vd = reinterpret_cast<half8 *>(p.v_tail + at);
                 kd[0] = kn[0]; kd[1] = kn[1];
@@ -314,23 +459,21 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
             quantise_tail<D>(p.v_tail + tail_off, p.v8 + row_off + (size_t)P0 * D, p.v_scale + (size_t)bh * p.nblk + blk, T, s_red);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads(); // and the block in the cache
+            request_scales(r);
+            request_k(r);
+            request_v(r);
         }
     }
 
     // The rotated query
     float qf[16];
-    if (has_chunk) {
-        load_input<16>(a.q, p.in_kind, in_off, inp_scale, p.in_kind == kInI32 ? a.wq_scale + h * D + e0 : nullptr, qf);
-        rotate_run<16>(qf, freq);
-    } else {
+    input_values(q_raw, kind, inp_scale, kind == kInI32 ? a.wq_scale + h * D + e0_in : nullptr, qf);
+    rotate_by(qf, fr);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) qf[i] = 0.f;
-    }
+    for (int i = 0; i < 16; ++i) qf[i] = has_chunk ? qf[i] : 0.f;
 
     const float scale = a.scale * kLog2e;
-    const float floor_m = kMaxFloor * kLog2e;
-    const float *mrow = HAS_MASK ? a.attn_mask + (size_t)q_pos * a.mask_ld : nullptr;
-    float m = floor_m, l = 0.f, lt = 0.f; // wave-uniform maximum; this lane group's sums over all rows / the tail rows
+    float m = kMaxFloor * kLog2e, l = 0.f, lt = 0.f; // wave-uniform maximum; this lane group's sums over all rows / the tail rows
     float o[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] = 0.f;
@@ -345,31 +488,11 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
         }
     };
 
-    // The tail: fp16 rows [P0, P], the newest from registers.  Two rows per lane group and trip.
-    if (owner && !fills) {
-        const int n = PROMPT ? ctx - P0 : P - P0; // rows to be read
-        const _Float16 *kt = p.k_tail + tail_off + e0, *vt = p.v_tail + tail_off + e0;
-        constexpr int UT = 2;
-        for (int r0 = wave * GPW * UT; r0 < n; r0 += kKv8Waves * GPW * UT) {
-            half8 kx[UT][2], vx[UT][2];
-            float s[UT], mk[UT];
-            bool ok[UT];
-#pragma unroll
-            for (int u = 0; u < UT; ++u) {
-                const int r = r0 + u * GPW + g;
-                ok[u] = r < n;
-                const size_t at = (size_t)min(r, n - 1) * D;
-                if (has_chunk) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        kx[u][c] = reinterpret_cast<const half8 *>(kt + at)[c];
-                        vx[u][c] = reinterpret_cast<const half8 *>(vt + at)[c];
-                    }
-                } else {
-                    kx[u][0] = kx[u][1] = vx[u][0] = vx[u][1] = half8{0, 0, 0, 0, 0, 0, 0, 0};
-                }
-                mk[u] = HAS_MASK ? mrow[P0 + min(r, n - 1)] * kLog2e : 0.f;
-            }
+    // The tail: fp16 rows [P0, P], the newest from registers.
+    if (has_tail) {
+        for (int r0 = wave * GPW * UT; r0 < n_tail; r0 += kKv8Waves * GPW * UT) {
+            if (r0 >= kKv8Waves * GPW * UT) request_tail(r0);
+            float s[UT];
 #pragma unroll
             for (int u = 0; u < UT; ++u) {
                 float acc = 0.f;
@@ -381,7 +504,8 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
             float top = -__builtin_inff();
 #pragma unroll
             for (int u = 0; u < UT; ++u) {
-                s[u] = ok[u] ? (HAS_MASK ? fmaf(s[u], scale, mk[u]) : s[u] * scale) : -__builtin_inff();
+                s[u] = HAS_MASK ? fmaf(s[u], scale, mt[u] * kLog2e) : s[u] * scale;
+                if (r0 + u * GPW + g >= n_tail) s[u] = -__builtin_inff();
                 top = fmaxf(top, s[u]);
             }
             raise(cross_max<LPR>(top));
@@ -396,21 +520,17 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
         }
         if (!PROMPT && wave == 0) { // the new row: every lane group has it, group 0 counts it
             float acc = 0.f;
-            if (has_chunk) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc = fmaf((float)kn[i / 8][i % 8], qf[i], acc);
-            }
+            for (int i = 0; i < 16; ++i) acc = fmaf((float)kn[i / 8][i % 8], qf[i], acc);
             acc = group_sum<LPR>(acc);
-            const float s = HAS_MASK ? fmaf(acc, scale, mrow[P] * kLog2e) : acc * scale;
+            const float s = HAS_MASK ? fmaf(acc, scale, mask_new) : acc * scale;
             raise(s);
             if (g == 0) {
                 const float e = __builtin_amdgcn_exp2f(s - m);
                 l += e;
                 lt += e;
-                if (has_chunk) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = fmaf(e, (float)vn[i / 8][i % 8], o[i]);
-                }
+                for (int i = 0; i < 16; ++i) o[i] = fmaf(e, (float)vn[i / 8][i % 8], o[i]);
             }
         }
     }
@@ -445,39 +565,31 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
     }
 
     // The byte rows
-    const __amdgpu_buffer_rsrc_t Kbuf = make_buffer(p.k8 + row_off), Vbuf = make_buffer(p.v8 + row_off);
-    const __amdgpu_buffer_rsrc_t Mbuf = make_buffer(HAS_MASK ? (const void *)mrow : (const void *)p.k8);
-    const float *ks_at = p.k_scale + (size_t)bh * p.nblk, *vs_at = p.v_scale + (size_t)bh * p.nblk;
-    const uint32_t lane_off = has_chunk ? (uint32_t)(g * D + e0) : kLaneOutOfRange;
-    const bool gather = !PROMPT && p.weights != nullptr;
-
-    auto trip = [&](int r, auto check_tag) __attribute__((always_inline)) {
-        constexpr bool CHECK = decltype(check_tag)::value;
-        u32x4 kv[U], vv[U];
-        float mk[U], ks[G::NS], vs[G::NS];
-        bool ok[U]; // uniform: a load instruction's rows are whole blocks' or whole parts of one
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            ok[u] = !CHECK || r + u * GPW < end8;
-            if constexpr (HAS_MASK)
-                mk[u] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(Mbuf, ok[u] ? (uint32_t)g * 4u : kLaneOutOfRange,
-                                                                                       (uint32_t)(r + u * GPW) * 4u, 0));
+    float gran_m = 0.f, gran_s = 0.f; // lane i: granule i of the current batch
+    float2 *const gran_at = gather ? p.granules + (size_t)bh * (L / GR) : nullptr;
+    float2 *const gran_lds = reinterpret_cast<float2 *>(s_merge_bytes);
+    const bool gran_local = direct && ctx <= LDS_GRANULES * GR;
+    int trip = 0, batch_row = r;
+    auto flush_granules = [&]() __attribute__((always_inline)) {
+        const int row = lane_row(batch_row);
+        if (row < min(r, end8)) { // of the trips that have been made (r: the next one)
+            if (gran_local) {
+                gran_lds[row / GR] = make_float2(gran_m, gran_s);
+            } else {
+                float *dst = reinterpret_cast<float *>(gran_at + row / GR);
+                store_partial<true>(dst, gran_m);
+                store_partial<true>(dst + 1, gran_s);
+            }
         }
+    };
+    while (r < end8) {
+        const int next = r + kKv8Waves * WT;
+        float s[U], ks[G::NG], vs[G::NG];
 #pragma unroll
-        for (int n = 0; n < G::NS; ++n) {
-            const int blk = min((r + 32 * n) >> p.t_shift, p.nblk - 1);
-            ks[n] = ks_at[blk];
-            vs[n] = !CHECK || r + 32 * n < end8 ? vs_at[blk] : 0.f; // (a block that was never written may have any scale)
+        for (int n = 0; n < G::NG; ++n) {
+            ks[n] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_lanes), trip * G::NG + n));
+            vs[n] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_lanes), trip * G::NG + n));
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            kv[u] = __builtin_amdgcn_raw_buffer_load_b128(Kbuf, ok[u] ? lane_off : kLaneOutOfRange, (uint32_t)(r + u * GPW) * (uint32_t)D, kLoadNonTemporal);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            vv[u] = __builtin_amdgcn_raw_buffer_load_b128(Vbuf, ok[u] ? lane_off : kLaneOutOfRange, (uint32_t)(r + u * GPW) * (uint32_t)D, kLoadNonTemporal);
-        __builtin_amdgcn_sched_barrier(0);
-
-        float s[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             int acc[3] = {0, 0, 0};
@@ -489,21 +601,49 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
             s[u] = fmaf((float)acc[2], 65536.f, (float)(acc[0] + (acc[1] << 8)));
         }
         group_sum_n<LPR, U>(s);
+        float mu[U];
+        if constexpr (HAS_MASK) {
+            if constexpr (MASK_QUAD) {
+                const float mq = mk[0] * kLog2e;
+                mu[0] = dpp_move<0x00>(mq); mu[1] = dpp_move<0x55>(mq); mu[2] = dpp_move<0xAA>(mq); mu[3] = dpp_move<0xFF>(mq);
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) mu[u] = mk[MASK_QUAD ? 0 : u] * kLog2e;
+            }
+        }
         float top = -__builtin_inff();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float f = qs * ks[u * GPW / 32];
-            s[u] = HAS_MASK ? fmaf(s[u], f, mk[u] * kLog2e) : s[u] * f;
-            if (CHECK && !ok[u]) s[u] = -__builtin_inff();
+            const float f = qs * ks[u * GPW / GR];
+            s[u] = HAS_MASK ? fmaf(s[u], f, mu[u]) : s[u] * f;
+            if (CHECK && r + u * GPW >= end8) s[u] = -__builtin_inff();
             top = fmaxf(top, s[u]);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        request_k(next); // (nothing is read behind the last row)
         raise(cross_max<LPR>(top));
         float e[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             e[u] = __builtin_amdgcn_exp2f(s[u] - m);
             l += e[u];
-            const float w = e[u] * vs[u * GPW / 32];
+        }
+        if (gather) {
+            constexpr int UG = U / G::NG; // load instructions per granule
+#pragma unroll
+            for (int n = 0; n < G::NG; ++n) { // (a granule is whole or absent: blocks are multiples of it)
+                float sum = 0.f;
+#pragma unroll
+                for (int u = 0; u < UG; ++u) sum += e[n * UG + u];
+                sum = cross_sum<LPR>(sum);
+                const bool mine = lane == trip * G::NG + n;
+                gran_m = mine ? m : gran_m;
+                gran_s = mine ? sum : gran_s;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float w = e[u] * vs[u * GPW / GR];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 o[4 * j + 0] = fmaf(w, byte_float<0>(vv[u][j]), o[4 * j + 0]);
@@ -512,26 +652,17 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
                 o[4 * j + 3] = fmaf(w, byte_float<3>(vv[u][j]), o[4 * j + 3]);
             }
         }
-        if (gather) {
-            constexpr int NG = WT / GR, UG = U / NG; // granules per trip, load instructions per granule
-#pragma unroll
-            for (int n = 0; n < NG; ++n) {
-                if (CHECK && !ok[n * UG]) continue; // a granule is whole or absent: T and the chunk are multiples of it
-                float sum = 0.f;
-#pragma unroll
-                for (int u = 0; u < UG; ++u) sum += e[n * UG + u];
-                sum = cross_sum<LPR>(sum);
-                float *dst = reinterpret_cast<float *>(p.granules + (size_t)bh * (L / GR) + r / GR + n);
-                if (lane == 0) {
-                    store_partial<true>(dst, m);
-                    store_partial<true>(dst + 1, sum);
-                }
-            }
+        __builtin_amdgcn_sched_barrier(0);
+        request_v(next);
+        r = next;
+        if (++trip == G::BATCH) { // (uniform)
+            if (gather) flush_granules();
+            trip = 0;
+            batch_row = r;
+            request_scales(r);
         }
-    };
-    int r = start + wave * WT;
-    for (; r + WT <= end8; r += kKv8Waves * WT) trip(r, std::false_type{});
-    if (r < end8) trip(r, std::true_type{});
+    }
+    if (gather) flush_granules();
 
     // Merge: lane groups in registers, waves through LDS.
 #pragma unroll
@@ -558,13 +689,16 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
         Lsum = fmaf(s_l[w], f[w], Lsum);
         Lt = fmaf(s_t[w], f[w], Lt);
     }
-    if (gather && owner && !fills && tid == 0) { // the open block's weight as its first granule
-        float *dst = reinterpret_cast<float *>(p.granules + (size_t)bh * (L / GR) + P0 / GR);
-        store_partial<true>(dst, M);
-        store_partial<true>(dst + 1, Lt);
+    if (gather && has_tail && tid == 0) { // the open block's weight as its first granule
+        if (gran_local) {
+            gran_lds[P0 / GR] = make_float2(M, Lt);
+        } else {
+            float *dst = reinterpret_cast<float *>(gran_at + P0 / GR);
+            store_partial<true>(dst, M);
+            store_partial<true>(dst + 1, Lt);
+        }
     }
     const size_t slot = (size_t)bh * a.split_cap + split;
-    const bool direct = PROMPT || a.direct;
     for (int d = tid; d < D; d += kKv8Waves * 64) {
         float O = 0.f;
 #pragma unroll
@@ -572,34 +706,37 @@ __global__ __launch_bounds__(kKv8Waves * 64) void kv8_attn_kernel(const Kv8Param
         if (direct) a.out[(PROMPT ? (size_t)bh * p.S + s_query : (size_t)bh) * D + d] = O / Lsum;
         else store_partial<true>(a.part_o + slot * D + d, O);
     }
-    if (PROMPT) return;
-    if (direct) {
-        if (gather) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads(); // every wave's granules are written
-            add_block_weights<D>(p, bh, P, M, Lsum, tid);
+    if constexpr (!PROMPT) {
+        if (direct) {
+            if (gather) {
+                if (!gran_local) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads(); // every wave's granules are written
+                if (gran_local) add_block_weights<D>(p, bh, P, M, Lsum, tid, [&](int i) __attribute__((always_inline)) { return gran_lds[i]; }, old_weight);
+                else add_block_weights<D>(p, bh, P, M, Lsum, tid, granule_loader(gran_at), old_weight);
+            }
+            return;
         }
-        return;
-    }
-    if (tid == 0) {
-        store_partial<true>(a.part_m + slot, M);
-        store_partial<true>(a.part_l + slot, Lsum);
-    }
-    if (!a.arrivals) return;
-    // Publish -> count -> merge, ordered as in the streaming kernel of the other cache types: device-coherent stores, a wait
-    // for their acknowledgement in every thread, the barrier, the device-scope count, the barrier, device-coherent loads.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    const int nsp = active_splits(a, P);
-    if (tid == 0) {
-        const int before = __hip_atomic_fetch_add(a.arrivals + bh, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = before == nsp - 1;
-        if (before == nsp - 1) __hip_atomic_store(a.arrivals + bh, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (s_last) {
-        const float2 ml = combine_partials<D, true>(a, bh, nsp, tid, s_merge);
-        if (gather) add_block_weights<D>(p, bh, P, ml.x, ml.y, tid);
+        if (tid == 0) {
+            store_partial<true>(a.part_m + slot, M);
+            store_partial<true>(a.part_l + slot, Lsum);
+        }
+        if (!a.arrivals) return;
+        // Publish -> count -> merge, ordered as in the streaming kernel of the other cache types: device-coherent stores, a
+        // wait for their acknowledgement in every thread, the barrier, the device-scope count, the barrier, device-coherent
+        // loads.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) {
+            const int before = __hip_atomic_fetch_add(a.arrivals + bh, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s_last = before == splits - 1;
+            if (before == splits - 1) __hip_atomic_store(a.arrivals + bh, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (s_last) {
+            if (gather && tid <= P >> p.t_shift) old_weight = p.weights[(size_t)bh * p.nblk + tid];
+            const float2 ml = combine_partials<D, true>(a, bh, splits, tid, *reinterpret_cast<CombineShared<D> *>(s_merge_bytes));
+            if (gather) add_block_weights<D>(p, bh, P, ml.x, ml.y, tid, granule_loader(gran_at), old_weight);
+        }
     }
 }
 
@@ -614,8 +751,11 @@ __global__ __launch_bounds__(kCombineThreads) void kv8_combine_kernel(const Kv8P
         for (int d = tid; d < D; d += kCombineThreads) p.a.out[(size_t)bh * D + d] = __builtin_nanf("");
         return;
     }
-    const float2 ml = combine_partials<D, false>(p.a, bh, active_splits(p.a, P), tid, sh);
-    if (p.weights) add_block_weights<D>(p, bh, P, ml.x, ml.y, tid);
+    const float2 ml = combine_partials<D, false>(p.a, bh, kv8_splits(p.a, p.T, P), tid, sh);
+    if (p.weights) {
+        const float old = tid <= P >> p.t_shift ? p.weights[(size_t)bh * p.nblk + tid] : 0.f;
+        add_block_weights<D>(p, bh, P, ml.x, ml.y, tid, granule_loader(p.granules + (size_t)bh * (p.a.L / Kv8Geometry<D>::GR)), old);
+    }
 }
 
 // ---------------------------------------------------------------- prompt phase: append

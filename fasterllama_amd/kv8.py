@@ -75,6 +75,7 @@ class KV8Attention:
         self.dtype, self.device = dtype, torch.device(device)
         if self.device.index is None:
             self.device = torch.device(self.device.type, torch.cuda.current_device())
+        self._index = self.device.index
         self.block_len, self.max_seq_len = block_len, max_seq_len
         self.shape = (batch_size, head_num, total_len, size_per_head)
         self.desc = capi.AttnDesc(batch_size, head_num, size_per_head, total_len,
@@ -95,55 +96,64 @@ class KV8Attention:
         """call(*args, stream) on torch's current stream of this object's device."""
         stream = torch.cuda.current_stream(self.device).cuda_stream
         if torch.cuda.current_device() == self.device.index:
-            capi.check(call(*args, stream))
+            status = call(*args, stream)
         else:
             with torch.cuda.device(self.device):
-                capi.check(call(*args, stream))
+                status = call(*args, stream)
+        if status:
+            capi.check(status)
 
     def _input(self, name: str, t: torch.Tensor, shape, dtype) -> int:
-        _need(t.dtype == dtype and tuple(t.shape) == shape and t.is_contiguous() and t.device == self.device,
-              f"{name} must be a contiguous {dtype} tensor {shape} on {self.device}")
+        if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != self._index:
+            _need(False, f"{name} must be a contiguous {dtype} tensor {shape} on {self.device}")
         return t.data_ptr()
 
     def _vector(self, name: str, t: torch.Tensor | None, dtype, numel: int) -> int | None:
         if t is None:
             return None
-        _need(t.dtype == dtype and t.numel() == numel and t.is_contiguous() and t.device == self.device,
-              f"{name} must hold {numel} contiguous {dtype} on {self.device}")
+        if t.dtype is not dtype or t.numel() != numel or not t.is_contiguous() or t.get_device() != self._index:
+            _need(False, f"{name} must hold {numel} contiguous {dtype} on {self.device}")
         return t.data_ptr()
 
     def _cache(self, cache: KV8Cache, shape=None) -> None:
-        _need(cache.shape == (shape or self.shape) and cache.block_len == self.block_len and cache.device == self.device,
-              f"the cache must be [B, H, L, D] = {shape or self.shape} in blocks of {self.block_len} on {self.device}")
+        if cache.shape != (shape or self.shape) or cache.block_len != self.block_len or cache.device != self.device:
+            B, H, L, D = shape or self.shape
+            _need(False, f"the cache must be [B, H, L, D] = {(B, H, L, D)} in blocks of {self.block_len} on {self.device}")
 
-    def _fill(self, q, k_new, v_new, seq_len, freq_cis, attn_mask, scales, out, out_shape, out_int8, out_scale):
+    def _fill(self, q, k_new, v_new, seq_len, freq_cis, rope_rows, attn_mask, last, scales, out, out_shape, out_int8, out_scale):
+        """Everything of io that both phases share; rope_rows: table rows the call uses (0: not known here), last: its last
+        row of the cache."""
         B, H, _, D = self.shape
         io, shape = self.io, (B, seq_len, H, D)
         dtype = self.dtype if scales is None else torch.int32
-        io.q, io.k_new, io.v_new = (self._input(n, t, shape, dtype) for n, t in (("q", q), ("k_new", k_new), ("v_new", v_new)))
-        _need(freq_cis.dtype == torch.float32 and freq_cis.dim() == 2 and freq_cis.shape[1] == D and freq_cis.is_contiguous()
-              and freq_cis.device == self.device, f"freq_cis must be a contiguous float32 table [rows, {D}] on {self.device}")
-        io.freq_cis = freq_cis.data_ptr()
+        io.q, io.k_new, io.v_new = self._input("q", q, shape, dtype), self._input("k_new", k_new, shape, dtype), self._input("v_new", v_new, shape, dtype)
+        rows = freq_cis.shape[0]
+        if rows < rope_rows:
+            _need(False, f"freq_cis has {rows} rows, the call uses {rope_rows}")
+        io.freq_cis = self._input("freq_cis", freq_cis, (rows, D), torch.float32)
         if attn_mask is None:
-            io.attn_mask, io.mask_ld = None, 0
+            io.attn_mask = None
         else:
-            _need(attn_mask.dtype == torch.float32 and attn_mask.dim() == 2 and attn_mask.stride(1) == 1
-                  and attn_mask.device == self.device, f"attn_mask must be float32 [rows, columns], columns contiguous, on {self.device}")
-            io.attn_mask, io.mask_ld = attn_mask.data_ptr(), 0 if attn_mask.shape[0] == 1 else attn_mask.stride(0)
-        s = scales or (None, None, None, None)
-        io.qkv_inp_scale = self._vector("qkv_inp_scale", s[0], torch.float32, B * seq_len)
-        io.q_weight_scale, io.k_weight_scale, io.v_weight_scale = (
-            self._vector(n, t, torch.float32, H * D) for n, t in zip(("q_weight_scale", "k_weight_scale", "v_weight_scale"), s[1:]))
+            if attn_mask.dtype is not torch.float32 or attn_mask.dim() != 2 or attn_mask.stride(1) != 1 or attn_mask.get_device() != self._index:
+                _need(False, f"attn_mask must be float32 [rows, columns], columns contiguous, on {self.device}")
+            n, m = attn_mask.shape
+            if m <= last or (n != 1 and n <= last):
+                _need(False, f"attn_mask is {n} x {m}, the call uses row and column {last}")
+            io.attn_mask, io.mask_ld = attn_mask.data_ptr(), 0 if n == 1 else attn_mask.stride(0)
+        if scales is None:
+            io.qkv_inp_scale = io.q_weight_scale = io.k_weight_scale = io.v_weight_scale = None
+        else:
+            io.qkv_inp_scale = self._vector("qkv_inp_scale", scales[0], torch.float32, B * seq_len)
+            io.q_weight_scale, io.k_weight_scale, io.v_weight_scale = (
+                self._vector(n, t, torch.float32, H * D) for n, t in zip(("q_weight_scale", "k_weight_scale", "v_weight_scale"), scales[1:]))
         if out is None and out_int8 is None:
             out = torch.empty(out_shape, dtype=torch.float32, device=self.device)
-        io.out = None if out is None else self._input("out", out, out_shape, torch.float32)
+            io.out = out.data_ptr()
+        else:
+            io.out = None if out is None else self._input("out", out, out_shape, torch.float32)
         io.out_int8 = self._vector("out_int8", out_int8, torch.int8, B * seq_len * H * D)
         io.out_scale = self._vector("out_scale", out_scale, torch.float32, B * seq_len)
         return out
-
-    @staticmethod
-    def _rows_fit(what: str, t: torch.Tensor | None, rows: int, columns: int | None = None) -> None:
-        _need(t is None or (t.shape[0] >= rows and (columns is None or t.shape[1] >= columns)), f"{what} is too small")
 
     def decode(self, q, k_new, v_new, cache: KV8Cache, freq_cis, start_pos: int = 0, attn_mask=None, start_pos_per_seq=None,
                max_start_pos: int = -1, rope_row: int = capi.FL_ATTN_ROPE_AT_POSITION, rope_row_per_seq=None, scales=None,
@@ -154,16 +164,14 @@ class KV8Attention:
         q/k/v_weight_scale) for int32 accumulators."""
         B, H, L, D = self.shape
         self._cache(cache)
-        out = self._fill(q, k_new, v_new, 1, freq_cis, attn_mask, scales, out, (B, H * D), out_int8, out_scale)
-        io = self.io
         last = start_pos if start_pos_per_seq is None else (L - 1 if max_start_pos < 0 else max_start_pos)
-        if attn_mask is not None:
-            self._rows_fit("attn_mask", attn_mask, 1 if io.mask_ld == 0 else last + 1, last + 1)
-        if rope_row_per_seq is None:  # (rows named on the device cannot be looked at here)
-            self._rows_fit("freq_cis", freq_cis, (last if rope_row < 0 else rope_row) + 1)
+        # (rows named on the device cannot be looked at here)
+        rope_rows = 0 if rope_row_per_seq is not None else (last if rope_row < 0 else rope_row) + 1
+        out = self._fill(q, k_new, v_new, 1, freq_cis, rope_rows, attn_mask, last, scales, out, (B, H * D), out_int8, out_scale)
+        io = self.io
         io.start_pos_per_seq = self._vector("start_pos_per_seq", start_pos_per_seq, torch.int32, B)
         io.start_pos, io.max_start_pos, io.rope_row = start_pos, max_start_pos, rope_row
-        io.flags, io.mask_tile_classes = capi.FL_ATTN_IO_WORKSPACE_READY, None
+        io.flags = capi.FL_ATTN_IO_WORKSPACE_READY
         self._enqueue(self.lib.fl_kv8_decode_forward, self._desc, cache.ref, self._io,
                       self._vector("rope_row_per_seq", rope_row_per_seq, torch.int32, B))
         return out
@@ -178,11 +186,9 @@ class KV8Attention:
         S = q.shape[1] if q.dim() == 4 else 0
         _need(0 < S <= self.max_seq_len, f"q is [B, S, H, D] with 1 <= S <= max_seq_len = {self.max_seq_len}")
         self._cache(cache)
-        out = self._fill(q, k_new, v_new, S, freq_cis, attn_mask, scales, out, (B, H, S, D), out_int8, out_scale)
+        out = self._fill(q, k_new, v_new, S, freq_cis, (start_pos if rope_row < 0 else rope_row) + S, attn_mask, start_pos + S - 1,
+                         scales, out, (B, H, S, D), out_int8, out_scale)
         io = self.io
-        if attn_mask is not None:
-            self._rows_fit("attn_mask", attn_mask, 1 if io.mask_ld == 0 else start_pos + S, start_pos + S)
-        self._rows_fit("freq_cis", freq_cis, (start_pos if rope_row < 0 else rope_row) + S)
         io.start_pos_per_seq = None
         io.start_pos, io.max_start_pos, io.rope_row, io.flags = start_pos, -1, rope_row, 0
         io.mask_tile_classes = None if mask_tile_classes is None else mask_tile_classes.data_ptr()
@@ -193,7 +199,8 @@ class KV8Attention:
         """The values of rows [0, rows): k, v [B,H,rows,D] in dtype; zeros from rows_per_seq[b] (int32 [B]) on."""
         B, H, _, D = self.shape
         self._cache(cache)
-        k, v = (torch.empty(B, H, max(rows, 0), D, dtype=self.dtype, device=self.device) for _ in range(2))
+        k = torch.empty(B, H, max(rows, 0), D, dtype=self.dtype, device=self.device)
+        v = torch.empty_like(k)
         self._enqueue(self.lib.fl_kv8_read, self._desc, cache.ref, rows, self._vector("rows_per_seq", rows_per_seq, torch.int32, B),
                       k.data_ptr(), v.data_ptr())
         return k, v
