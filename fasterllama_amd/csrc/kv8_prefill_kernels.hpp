@@ -89,54 +89,59 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
         else return (uint32_t)(c0 + i) << 8 | 0x55u;
     };
 
-    // global -> registers (fetch), registers -> LDS (commit) of a key tile: bytes, or fp16 rows of the tail (twice as many
-    // loads), whose rows behind the context arrive as zeros.
+    // global -> registers (fetch), registers -> LDS (commit) of a key tile.  A tile of the tail — fp16 rows, twice the loads, the
+    // last few tiles of the context — is loaded where it is committed: registers for both kinds would have to be merged
+    // behind the request, and the merge waits for the loads.  Its rows behind the context become zeros.
     const size_t row_off = (size_t)bh * L * D, tail_off = (size_t)bh * p.T * D;
-    u32x4 stage[LPT], stage_hi[LPT]; // (stage_hi: tail rows only)
+    const float *ks_at = p.k_scale + (size_t)bh * p.nblk, *vs_at = p.v_scale + (size_t)bh * p.nblk;
+    u32x4 stage[LPT];
+    float stage_ks = 1.f, stage_vs = 1.f; // the tile's scales travel with it
     auto fetch = [&](int t) __attribute__((always_inline)) {
-        const bool tail = t * BN >= ctx8; // uniform
+        if (t * BN >= ctx8) return; // uniform
+        stage_ks = ks_at[t * BN >> p.t_shift];
+        stage_vs = vs_at[t * BN >> p.t_shift];
 #pragma unroll
         for (int j = 0; j < LPT; ++j) {
             const bool is_v = (wave + 4 * j) * 64 >= NCH; // uniform: NCH is a multiple of 64
             const int i = tid + j * 256 - (is_v ? NCH : 0);
-            const int r = i / CPR8, e0 = (i % CPR8) * 16;
-            if (2 * NCH % 256 == 0 || (wave + 4 * j) * 64 < 2 * NCH) {
-                if (!tail) {
-                    stage[j] = *reinterpret_cast<const u32x4 *>((is_v ? p.v8 : p.k8) + row_off + (size_t)t * (BN * D) + (r * D + e0));
-                } else {
-                    const int row = t * BN + r - ctx8;
-                    const _Float16 *src = (is_v ? p.v_tail : p.k_tail) + tail_off + (size_t)min(row, ctx - ctx8 - 1) * D + e0;
-                    stage[j] = *reinterpret_cast<const u32x4 *>(src);
-                    stage_hi[j] = *reinterpret_cast<const u32x4 *>(src + 8);
-                    if (row >= ctx - ctx8) stage[j] = stage_hi[j] = u32x4{0, 0, 0, 0};
-                }
-            }
+            if (2 * NCH % 256 == 0 || (wave + 4 * j) * 64 < 2 * NCH)
+                stage[j] = *reinterpret_cast<const u32x4 *>((is_v ? p.v8 : p.k8) + row_off + (size_t)t * (BN * D) + i * 16);
         }
     };
+    float next_ks = 1.f, next_vs = 1.f;
     auto commit = [&](int t, int buf) __attribute__((always_inline)) {
         const bool tail = t * BN >= ctx8;
+        next_ks = tail ? 1.f : __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(stage_ks))); // tail rows are values
+        next_vs = tail ? 1.f : __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(stage_vs)));
 #pragma unroll
         for (int j = 0; j < LPT; ++j) {
             const bool is_v = (wave + 4 * j) * 64 >= NCH;
             const int i = tid + j * 256 - (is_v ? NCH : 0);
             const int r = i / CPR8, e0 = (i % CPR8) * 16;
             if (2 * NCH % 256 == 0 || (wave + 4 * j) * 64 < 2 * NCH) {
-                half8 y0, y1;
+                half8 *dst = reinterpret_cast<half8 *>(is_v ? &sV[buf][r][e0] : &sK[buf][r][e0]);
                 if (!tail) {
                     half2v h[8];
                     widen4(stage[j][0], h[0], h[1]);
                     widen4(stage[j][1], h[2], h[3]);
                     widen4(stage[j][2], h[4], h[5]);
                     widen4(stage[j][3], h[6], h[7]);
+                    half8 y0, y1;
 #pragma unroll
                     for (int c = 0; c < 8; ++c) { y0[c] = h[c / 2][c % 2]; y1[c] = h[4 + c / 2][c % 2]; }
+                    dst[0] = y0;
+                    dst[1] = y1;
                 } else {
-                    y0 = __builtin_bit_cast(half8, stage[j]);
-                    y1 = __builtin_bit_cast(half8, stage_hi[j]);
+                    const int row = t * BN + r - ctx8;
+                    half8 y0 = half8{0, 0, 0, 0, 0, 0, 0, 0}, y1 = y0;
+                    if (row < ctx - ctx8) {
+                        const half8 *src = reinterpret_cast<const half8 *>((is_v ? p.v_tail : p.k_tail) + tail_off + (size_t)row * D + e0);
+                        y0 = src[0];
+                        y1 = src[1];
+                    }
+                    dst[0] = y0;
+                    dst[1] = y1;
                 }
-                half8 *dst = reinterpret_cast<half8 *>(is_v ? &sV[buf][r][e0] : &sK[buf][r][e0]);
-                dst[0] = y0;
-                dst[1] = y1;
             }
         }
     };
@@ -296,7 +301,6 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     float m = kMaxFloor * kLog2e, l = 0.f;
     uint32_t vref = 0u; // bits of the power of two that the output accumulators are in units of (uniform); 0: none yet
     const int vrow = 4 * hf + ((lane & 15) >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    const float *ks_at = p.k_scale + (size_t)bh * p.nblk, *vs_at = p.v_scale + (size_t)bh * p.nblk;
 #pragma unroll
     for (int c = 0; c < NC; ++c) asm volatile("" : "+v"(qhi[c]), "+v"(qlo[c]));
 
@@ -316,11 +320,7 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
         auto tile_step = [&](int i, auto buf_tag) __attribute__((always_inline)) {
             constexpr int buf = decltype(buf_tag)::value;
             const int t = (int)(e0 >> 8), k0 = t * BN;
-            float ks = 1.f, vs = 1.f; // tail rows are values themselves
-            if (k0 < ctx8) {
-                ks = ks_at[k0 >> p.t_shift];
-                vs = vs_at[k0 >> p.t_shift];
-            }
+            const float ks = next_ks, vs_tile = next_vs; // committed with tile t
             __syncthreads(); // tile t is visible; every wave is done with the other buffer
             uint32_t tc = kTileZero;
             if constexpr (HAS_MASK) tc = __builtin_amdgcn_readfirstlane((e0 >> (2 * wave)) & 3u);
@@ -341,12 +341,35 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
                 floatx16 st;
 #pragma unroll
                 for (int v = 0; v < 16; ++v) st[v] = 0.f;
+                // Operands are read from LDS one step ahead of the products that use them, the scheduler held to it: left alone
+                // it reads them right before, and every few products wait out an LDS round trip.
+                half8 kc[2][2];
+                auto k_stage = [&](int which, int c) __attribute__((always_inline)) {
+                    kc[which][0] = *reinterpret_cast<const half8 *>(&sK[buf][qi][16 * c + 8 * hf]);
+                    kc[which][1] = *reinterpret_cast<const half8 *>(&sK[buf][qi][16 * (c + 1) + 8 * hf]);
+                };
+                k_stage(0, 0);
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const half8 ka = *reinterpret_cast<const half8 *>(&sK[buf][qi][16 * c + 8 * hf]);
-                    st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qlo[c], st, 0, 0, 0);
-                    st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qhi[c], st, 0, 0, 0);
+                for (int c = 0; c < NC; c += 2) {
+                    if (c + 2 < NC) k_stage((c / 2 + 1) & 1, c + 2);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int cc = 0; cc < 2; ++cc) {
+                        st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kc[(c / 2) & 1][cc], qlo[c + cc], st, 0, 0, 0);
+                        st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kc[(c / 2) & 1][cc], qhi[c + cc], st, 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                half4 vst[2][4];
+                auto v_stage = [&](int which, int dt) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        vst[which][2 * u] = lds_read_tr16(&sV[buf][16 * u + vrow][32 * dt + vcol]);
+                        vst[which][2 * u + 1] = lds_read_tr16(&sV[buf][16 * u + 8 + vrow][32 * dt + vcol]);
+                    }
+                };
+                v_stage(0, 0);
+                __builtin_amdgcn_sched_barrier(0);
                 float cs = qc * ks; // raw product -> base-2 score
                 if (special) {
 #pragma unroll
@@ -362,17 +385,17 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
                     cs = 1.f;
                 }
                 // The accumulators' unit: a power of two no smaller than any block's scale so far.
-                if (vs == 0.f) vs = 1.f; // a block of zeros
+                const float vs = vs_tile == 0.f ? 1.f : vs_tile; // a block of zeros
                 const uint32_t vbits = __builtin_amdgcn_readfirstlane((__float_as_uint(vs) + 0x7fffffu) & 0xff800000u);
                 if (vbits > vref) { // uniform
-                    const float down = __uint_as_float(vref) / __uint_as_float(vbits);
+                    const float down = __uint_as_float(vref) * __uint_as_float(0x7f000000u - vbits); // (reciprocal of a power of two)
                     vref = vbits;
 #pragma unroll
                     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
                         for (int v = 0; v < 16; ++v) ot[dt][v] *= down;
                 }
-                const float lr = __builtin_amdgcn_logf(vs / __uint_as_float(vref)) + kKv8WeightExp; // log2
+                const float lr = __builtin_amdgcn_logf(vs * __uint_as_float(0x7f000000u - vref)) + kKv8WeightExp; // log2
                 const float mx = fmaxf(m, cross_half_max(max16(st)) * cs);
                 if (__ballot(mx > m + kLazyMax) != 0ull) { // wave-uniform
                     const float alpha = __builtin_amdgcn_exp2f(m - mx);
@@ -385,33 +408,38 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
                 }
                 const float nb = lr - m;
                 half8 ph[2], pl[2];
-                float sum = 0.f;
+                float sum0 = 0.f, sum1 = 0.f;
+                float minus1 = -1.0f; // opaque, so that e - h stays one mixed-precision FMA instead of a conversion and a subtraction
+                asm volatile("" : "+s"(minus1));
 #pragma unroll
                 for (int v = 0; v < 16; v += 2) {
-                    float2v e;
+                    float2v e, rem;
                     e[0] = __builtin_amdgcn_exp2f(fmaf(st[v], cs, nb));
                     e[1] = __builtin_amdgcn_exp2f(fmaf(st[v + 1], cs, nb));
-                    sum += e[0];
-                    sum += e[1];
+                    sum0 += e[0];
+                    sum1 += e[1];
                     const half2v h = __builtin_convertvector(e, half2v);
-                    ph[v / 8][v % 8] = h[0];
-                    ph[v / 8][v % 8 + 1] = h[1];
-                    pl[v / 8][v % 8] = (_Float16)fmaf(-(float)h[0], 1.0f, e[0]);
-                    pl[v / 8][v % 8 + 1] = (_Float16)fmaf(-(float)h[1], 1.0f, e[1]);
+                    rem[0] = fmaf((float)h[0], minus1, e[0]); // exact
+                    rem[1] = fmaf((float)h[1], minus1, e[1]);
+                    const half2v r = __builtin_convertvector(rem, half2v);
+                    ph[v / 8][v % 8] = h[0]; ph[v / 8][v % 8 + 1] = h[1];
+                    pl[v / 8][v % 8] = r[0]; pl[v / 8][v % 8 + 1] = r[1];
                 }
-                l = fmaf(sum, __builtin_amdgcn_exp2f(-lr), l);
+                l = fmaf(sum0 + sum1, __builtin_amdgcn_exp2f(-lr), l);
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt) {
+                    if (dt + 1 < NDT) v_stage((dt + 1) & 1, dt + 1);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const half4 lo = lds_read_tr16(&sV[buf][16 * u + vrow][32 * dt + vcol]);
-                        const half4 hi = lds_read_tr16(&sV[buf][16 * u + 8 + vrow][32 * dt + vcol]);
+                        const half4 lo = vst[dt & 1][2 * u], hi = vst[dt & 1][2 * u + 1];
                         half8 va;
                         va[0] = lo[0]; va[1] = lo[1]; va[2] = lo[2]; va[3] = lo[3];
                         va[4] = hi[0]; va[5] = hi[1]; va[6] = hi[2]; va[7] = hi[3];
                         ot[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[u], ot[dt], 0, 0, 0);
                         ot[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], ot[dt], 0, 0, 0);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             e0 = e1;
