@@ -21,6 +21,11 @@ def _need(ok: bool, what: str) -> None:
         raise capi.FlAttnError(capi.FL_ATTN_ERR_ARGUMENT, what)
 
 
+# The handle of torch's current stream.  A decode step of a small batch takes less time on the GPU than its call on the host, and
+# building a Stream object for its handle is a sixth of that call; the public way serves where torch lacks the short one.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class KV8Cache:
     """The arrays of one layer: k, v int8 [B,H,L,D]; k_scale, v_scale float32 [B,H,L/block_len]; k_tail, v_tail float16
     [B,H,block_len,D]; weights float32 [B,H,L/block_len] or None."""
@@ -91,11 +96,13 @@ class KV8Attention:
             stream.synchronize()  # the counters are zero for whatever stream the calls are made on
         self.io = capi.AttnIO(workspace=self.workspace.data_ptr(), workspace_bytes=n.value)
         self._io = C.byref(self.io)
+        self.evict_args = capi.Kv8EvictArgs()
+        self._evict_args = C.byref(self.evict_args)
 
     def _enqueue(self, call, *args) -> None:
         """call(*args, stream) on torch's current stream of this object's device."""
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        if torch.cuda.current_device() == self.device.index:
+        stream = _raw_stream(self._index)
+        if torch.cuda.current_device() == self._index:
             status = call(*args, stream)
         else:
             with torch.cuda.device(self.device):
@@ -216,8 +223,9 @@ class KV8Attention:
         _need(cache.weights is not None and to.weights is not None, "the caches must have weights")
         kept = torch.empty(B, H, max(keep_blocks, 0), dtype=torch.int32, device=self.device)
         rows_out = torch.empty(B, dtype=torch.int32, device=self.device)
-        args = capi.Kv8EvictArgs(rows=rows, rows_per_seq=self._vector("rows_per_seq", rows_per_seq, torch.int32, B),
-                                 keep_blocks=keep_blocks, recent_blocks=recent_blocks, to_total_len=to.shape[2],
-                                 kept=kept.data_ptr(), rows_out=rows_out.data_ptr())
-        self._enqueue(self.lib.fl_kv8_evict, self._desc, cache.ref, to.ref, C.byref(args))
+        args = self.evict_args
+        args.rows, args.rows_per_seq = rows, self._vector("rows_per_seq", rows_per_seq, torch.int32, B)
+        args.keep_blocks, args.recent_blocks, args.to_total_len = keep_blocks, recent_blocks, to.shape[2]
+        args.kept, args.rows_out = kept.data_ptr(), rows_out.data_ptr()
+        self._enqueue(self.lib.fl_kv8_evict, self._desc, cache.ref, to.ref, self._evict_args)
         return kept, rows_out
