@@ -134,12 +134,14 @@ __device__ __forceinline__ _Float16 stored_half(float x)
 
 // 127 / absmax; 0 for a block of zeros
 __device__ __forceinline__ float quant_factor(float absmax) { return absmax > 0.f ? 127.0f / absmax : 0.f; }
-// |x * factor| < 127.5 by construction: no clamp
-__device__ __forceinline__ int quantise(float x, float factor) { return (int)rintf(__fmul_rn(x, factor)); }
-
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d)
+// Four values as bytes.  |x * factor| < 127.5 by construction: no clamp.  The product is rounded to FP32, then adding 1.5 * 2^23
+// rounds it to the nearest-even integer, whose low byte is the sum's low byte.
+__device__ __forceinline__ uint32_t quantise4(_Float16 a, _Float16 b, _Float16 c, _Float16 d, float factor)
 {
-    return ((uint32_t)a & 0xffu) | ((uint32_t)b & 0xffu) << 8 | ((uint32_t)c & 0xffu) << 16 | (uint32_t)d << 24;
+    constexpr float kShift = 12582912.0f;
+    const uint32_t qa = __float_as_uint(__fmul_rn((float)a, factor) + kShift), qb = __float_as_uint(__fmul_rn((float)b, factor) + kShift);
+    const uint32_t qc = __float_as_uint(__fmul_rn((float)c, factor) + kShift), qd = __float_as_uint(__fmul_rn((float)d, factor) + kShift);
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(qd, qc, 0x0c0c0400u), __builtin_amdgcn_perm(qb, qa, 0x0c0c0400u), 0x05040100u);
 }
 
 template <int I>
@@ -261,8 +263,8 @@ __device__ __forceinline__ void quantise_tail(const _Float16 *tail, int8_t *rows
     for (int i = tid; i < n8; i += kKv8Waves * 64) {
         const half8 x = src[i];
         uint2 o;
-        o.x = pack4(quantise((float)x[0], f), quantise((float)x[1], f), quantise((float)x[2], f), quantise((float)x[3], f));
-        o.y = pack4(quantise((float)x[4], f), quantise((float)x[5], f), quantise((float)x[6], f), quantise((float)x[7], f));
+        o.x = quantise4(x[0], x[1], x[2], x[3], f);
+        o.y = quantise4(x[4], x[5], x[6], x[7], f);
         reinterpret_cast<uint2 *>(rows8)[i] = o;
     }
     if (tid == 0) *scale_at = absmax / 127.0f;
@@ -901,8 +903,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(const Kv8Params p)
             if (!EXACT && i >= T * CPR) continue;
             const half8 x = KEEP ? kept[KEEP ? n : 0] : chunk(i);
             uint2 o;
-            o.x = pack4(quantise((float)x[0], f), quantise((float)x[1], f), quantise((float)x[2], f), quantise((float)x[3], f));
-            o.y = pack4(quantise((float)x[4], f), quantise((float)x[5], f), quantise((float)x[6], f), quantise((float)x[7], f));
+            o.x = quantise4(x[0], x[1], x[2], x[3], f);
+            o.y = quantise4(x[4], x[5], x[6], x[7], f);
             dst[i] = o;
         }
         if (tid == 0) (is_v ? p.v_scale : p.k_scale)[(size_t)bh * p.nblk + blk] = absmax / 127.0f;
