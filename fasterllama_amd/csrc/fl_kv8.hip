@@ -188,7 +188,7 @@ hipError_t launch_prompt(const Kv8PromptParams &pp, hipStream_t stream)
         return launch(flattn::kv8_attn_kernel<D, false, true>, grid, block, stream, p);
     } else {
         const unsigned qblocks = (unsigned)((p.S + flattn::kPrefillQueriesPerBlock - 1) / flattn::kPrefillQueriesPerBlock);
-        if (p.a.attn_mask && !pp.f.class_table) { // no table of the whole mask at hand: classify the rows of this call
+        if (p.a.attn_mask && !pp.f.class_table && pp.f.tile_class) { // no table of the whole mask at hand: classify the rows of this call
             const int ktiles = (p.a.start_pos + p.S + flattn::kPrefillKeysPerStep - 1) / flattn::kPrefillKeysPerStep;
             e = launch(flattn::prefill_mask_classify_kernel, dim3((unsigned)ktiles, qblocks), dim3(256), stream, pp.f, ktiles);
             if (e != hipSuccess) return e;
@@ -197,10 +197,16 @@ hipError_t launch_prompt(const Kv8PromptParams &pp, hipStream_t stream)
         e = p.a.attn_mask ? launch(flattn::kv8_prefill_attn_kernel<D, true>, grid, block, stream, pp)
                           : launch(flattn::kv8_prefill_attn_kernel<D, false>, grid, block, stream, pp);
         if (e != hipSuccess || !p.stats) return e;
-        const dim3 wgrid((unsigned)((p.a.start_pos + p.S + p.T - 1) / p.T) * bh);
-        if (p.T == 32) return launch(flattn::kv8_prompt_weights_kernel<D, 32>, wgrid, block, stream, pp);
-        if (p.T == 64) return launch(flattn::kv8_prompt_weights_kernel<D, 64>, wgrid, block, stream, pp);
-        return launch(flattn::kv8_prompt_weights_kernel<D, 128>, wgrid, block, stream, pp);
+        // Query streams per workgroup of the block weights (see the kernel).  More streams, more and shorter workgroups, but each
+        // reads the operands for fewer keys: split until there are four workgroups per compute unit (under a causal mask the
+        // first keys' workgroups see every query, and with two per unit they finish last), not below four query blocks
+        // per stream; a workgroup's 256 / NQ keys are whole blocks.  The whole call, in us, for NQ = 1 / 2 / 4, D = 128:
+        //   32 heads, 4096 queries, all counted  646 / 602 / 621     B=8, 32 heads, 1024, the last 64   234 / 244 / 264
+        //   B=3, 5 heads (D = 96), 333, all       46 / 40 / 37
+        const int ctx = p.a.start_pos + p.S;
+        int NQ = 1;
+        while (NQ < 4 && 2 * NQ * p.T <= 256 && 4 * NQ < pp.kept_blocks && (int64_t)((ctx + 256 / NQ - 1) / (256 / NQ)) * bh < 4 * (int64_t)device_cus()) NQ *= 2;
+        return launch(flattn::kv8_prompt_weights_kernel<D>, dim3((unsigned)((ctx + 256 / NQ - 1) / (256 / NQ)) * bh), block, stream, pp, NQ);
     }
 }
 
@@ -363,7 +369,7 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
     Kv8PromptParams pp{};
     flattn::PrefillParams &f = pp.f;
     f.attn_mask = io.attn_mask; f.mask_ld = io.mask_ld;
-    f.tile_class = reinterpret_cast<uint32_t *>(ws + w.tile_class);
+    if (io.start_pos + seq_len > flattn::kUnclassifiedKeys) f.tile_class = reinterpret_cast<uint32_t *>(ws + w.tile_class);
     f.B = desc->batch_size; f.H = desc->head_num; f.L = L; f.S = seq_len; f.start_pos = io.start_pos;
     if (io.mask_tile_classes && io.attn_mask && io.mask_ld >= L && io.start_pos % 32 == 0) {
         if ((reinterpret_cast<uintptr_t>(io.mask_tile_classes) & 3u) != 0) return FL_ATTN_ERR_ALIGNMENT; // read a word at a time

@@ -41,6 +41,19 @@ __device__ __forceinline__ void widen4(uint32_t x, half2v &lo, half2v &hi)
     hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off;
 }
 
+// Classes of a key tile for the four 32-query sub-blocks of a 128-query block.  A short context is not classified (a launch of
+// its own costs more than reading its mask): every tile is kTileMixed, that of a sub-block behind the prompt kTileSkip.
+constexpr int kUnclassifiedKeys = 128;
+__device__ __forceinline__ uint32_t prompt_class_word(const PrefillParams &f, int qb, int t, int NT)
+{
+    if (f.tile_class || f.class_table) return tile_class_word(f, qb, t, NT);
+    uint32_t w = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (qb * kPrefillQueriesPerBlock + 32 * k < f.S) w |= kTileMixed << (8 * k);
+    return w;
+}
+
 __device__ __forceinline__ void wave_lds_sync() // orders this wave's LDS writes and reads
 {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -150,7 +163,7 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     fetch(0); // a guess at the first listed tile: right without a mask and under every causal one
     uint32_t w_first = 0;
     if constexpr (HAS_MASK) {
-        if (tid < first_c1) w_first = tile_class_word(pf, qb, tid, NT);
+        if (tid < first_c1) w_first = prompt_class_word(pf, qb, tid, NT);
     }
 
     // The rotated queries as fp16 pairs in operand layout, by way of LDS: every wave its own 32 (see the fp16 caches'
@@ -483,47 +496,65 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
 }
 
 // Block weights of a prompt: weights[b,h,blk] (+)= sum over the last weight_queries queries and the block's rows of
-// 2^(s' - m') / l, with the operands and statistics the attention kernel left.  grid = blocks * B*H, block = 256.  A wave keeps
-// 32 keys of the block in registers as operands and takes every (128 / T)-th 32-query block; the sum is formed in one order,
-// so it is the same from run to run.
-template <int D, int T>
-__global__ __launch_bounds__(256) void kv8_prompt_weights_kernel(const Kv8PromptParams pp)
+// 2^(s' - m') / l, with the operands and statistics the attention kernel left.  Two products' worth of matrix instructions per
+// query and key; what bounds it is reading the queries' operands, 16 KB per 32 of them at D = 128.  A wave keeps 64 keys in
+// registers, and the four waves of a workgroup are 4 / NQ groups of keys times NQ streams of queries: with NQ = 1 they read
+// the same operands together, with NQ = 4 a workgroup is done sooner, where there are few of them.  grid = ceil(keys / (256 / NQ))
+// * B*H, block = 256.  Sums are formed in one order, so they are the same from run to run.
+template <int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 8)))
+void kv8_prompt_weights_kernel(const Kv8PromptParams pp, int NQ)
 {
-    constexpr int NC = D / 16, NTB = T / 32, NQ = 4 / NTB; // key tiles of a block, waves that share a key tile
-    __shared__ float s_sum[4];
+    constexpr int NC = D / 16, KT = 2;
+    __shared__ float s_sum[4][KT];
     const Kv8Params &p = pp.k;
     const Params &a = p.a;
-    const int S = p.S, P = a.start_pos, ctx = P + S, NT = (ctx + 31) / 32;
-    const int nb = (ctx + T - 1) / T;
-    const int blk = blockIdx.x % nb, bh = blockIdx.x / nb;
+    const int S = p.S, P = a.start_pos, T = p.T, ctx = P + S, ctx8 = ctx & ~(T - 1), NT = (ctx + 31) / 32;
+    const int keys = 256 / NQ, groups = (ctx + keys - 1) / keys;
+    const int wg_key = blockIdx.x % groups * keys, bh = blockIdx.x / groups;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 31, hf = lane >> 5;
-    const int k0 = blk * T + 32 * (wave / NQ); // this wave's first key
-    const bool open = blk * T + T > ctx;
-    const float ks = open ? 1.f : p.k_scale[(size_t)bh * p.nblk + blk];
-    half8 ka[NC]; // key k0 + qi, elements 16c + 8hf ..
+    const int key0 = wg_key + wave / NQ * (32 * KT); // this wave's first key
+    half8 ka[KT][NC]; // key key0 + 32 t + qi, elements 16c + 8hf ..
+    float ks[KT];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        if (open) {
-            half8 z = half8{0, 0, 0, 0, 0, 0, 0, 0};
-            if (k0 + qi < ctx) z = *reinterpret_cast<const half8 *>(p.k_tail + ((size_t)bh * T + (k0 + qi - blk * T)) * D + 16 * c + 8 * hf);
-            ka[c] = z;
-        } else {
-            const uint2 x = *reinterpret_cast<const uint2 *>(p.k8 + ((size_t)bh * a.L + k0 + qi) * D + 16 * c + 8 * hf);
-            half2v h[4];
-            widen4(x.x, h[0], h[1]);
-            widen4(x.y, h[2], h[3]);
+    for (int t = 0; t < KT; ++t) {
+        const int k0 = key0 + 32 * t, row = k0 + qi;
+        ks[t] = 1.f;
+        if (k0 < ctx8) {
+            ks[t] = p.k_scale[(size_t)bh * p.nblk + (k0 >> p.t_shift)];
+            const int8_t *src = p.k8 + ((size_t)bh * a.L + row) * D + 8 * hf;
+            uint2 x[NC];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ka[c][i] = h[i / 2][i % 2];
+            for (int c = 0; c < NC; ++c) x[c] = *reinterpret_cast<const uint2 *>(src + 16 * c);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                half2v h[4];
+                widen4(x[c].x, h[0], h[1]);
+                widen4(x[c].y, h[2], h[3]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ka[t][c][i] = h[i / 2][i % 2];
+            }
+        } else { // the tail, zeros behind it
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                ka[t][c] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+                if (row < ctx) ka[t][c] = *reinterpret_cast<const half8 *>(p.k_tail + ((size_t)bh * T + (row - ctx8)) * D + 16 * c + 8 * hf);
+            }
         }
     }
     const int first_query = S - p.weight_queries;
-    float sum = 0.f;
-    for (int block = k0 < ctx ? wave % NQ : pp.kept_blocks; block < pp.kept_blocks; block += NQ) {
+    float sum[KT] = {0.f, 0.f};
+    for (int block = key0 < ctx ? wave % NQ : pp.kept_blocks; block < pp.kept_blocks; block += NQ) {
         const int q0 = (pp.first_block + block) * 32;
-        uint32_t cls = kTileZero;
-        if (a.attn_mask) cls = (tile_class_word(pp.f, q0 / kPrefillQueriesPerBlock, k0 / 32, NT) >> (8 * (q0 / 32 % 4))) & 0xffu;
-        cls = __builtin_amdgcn_readfirstlane(cls);
-        if (cls == kTileSkip) continue;
+        uint32_t cls[KT];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            cls[t] = kTileSkip;
+            if (key0 + 32 * t < ctx)
+                cls[t] = a.attn_mask ? (prompt_class_word(pp.f, q0 / kPrefillQueriesPerBlock, key0 / 32 + t, NT) >> (8 * (q0 / 32 % 4))) & 0xffu : kTileZero;
+            cls[t] = __builtin_amdgcn_readfirstlane(cls[t]);
+        }
+        if (cls[0] == kTileSkip && cls[1] == kTileSkip) continue;
         const size_t kept = (size_t)bh * pp.kept_blocks + block;
         const half8 *src = pp.q_pairs + kept * (2 * NC * 64) + lane;
         half8 qhi[NC], qlo[NC];
@@ -534,41 +565,54 @@ __global__ __launch_bounds__(256) void kv8_prompt_weights_kernel(const Kv8Prompt
         }
         const int q = q0 + qi, q_in = min(q, S - 1);
         const float2 ml = p.stats[(size_t)bh * S + q_in];
-        const float cs = pp.q_factor[kept * 32 + qi] * ks;
-        floatx16 st;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) st[v] = 0.f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[c], qlo[c], st, 0, 0, 0);
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[c], qhi[c], st, 0, 0, 0);
-        }
-        if (cls >= kTileMixed || k0 + 32 > ctx) { // uniform
-            const float *mrow = a.attn_mask + (size_t)(P + q_in) * a.mask_ld;
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int key = 8 * (v / 4) + 4 * hf + (v % 4);
-                float x = st[v] * cs;
-                if (cls == kTileMixed) x = fmaf(mrow[min(k0 + key, ctx - 1)], kLog2e, x);
-                st[v] = (cls == kTileDiag && key > qi) || k0 + key >= ctx ? -__builtin_inff() : x - ml.x;
-            }
-        } else {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) st[v] = fmaf(st[v], cs, -ml.x);
-        }
-        float part = 0.f;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) part += __builtin_amdgcn_exp2f(st[v]);
+        const float factor = pp.q_factor[kept * 32 + qi];
         // a query of the call that counts, and that saw a key
-        if (q >= first_query && q < S && ml.y > 0.f) sum += part / ml.y;
+        const float rl = q >= first_query && q < S && ml.y > 0.f ? 1.0f / ml.y : 0.f;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            if (cls[t] == kTileSkip) continue;
+            const int k0 = key0 + 32 * t;
+            const float cs = factor * ks[t];
+            floatx16 st;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) st[v] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[t][c], qlo[c], st, 0, 0, 0);
+                st = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[t][c], qhi[c], st, 0, 0, 0);
+            }
+            if (cls[t] >= kTileMixed || k0 + 32 > ctx) { // uniform
+                const float *mrow = a.attn_mask + (size_t)(P + q_in) * a.mask_ld;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int key = 8 * (v / 4) + 4 * hf + (v % 4);
+                    float x = st[v] * cs;
+                    if (cls[t] == kTileMixed) x = fmaf(mrow[min(k0 + key, ctx - 1)], kLog2e, x);
+                    st[v] = (cls[t] == kTileDiag && key > qi) || k0 + key >= ctx ? -__builtin_inff() : x - ml.x;
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) st[v] = fmaf(st[v], cs, -ml.x);
+            }
+            float part = 0.f;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) part += __builtin_amdgcn_exp2f(st[v]);
+            if (rl > 0.f) sum[t] = fmaf(part, rl, sum[t]);
+        }
     }
-    sum = wave_sum(sum);
-    if (lane == 0) s_sum[wave] = sum;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        sum[t] = wave_sum(sum[t]);
+        if (lane == 0) s_sum[wave][t] = sum[t];
+    }
     __syncthreads();
-    if (tid == 0) {
-        const float w = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-        float *dst = p.weights + (size_t)bh * p.nblk + blk;
-        *dst = blk * T >= P ? w : *dst + w;
+    const int row0 = wg_key + tid * T; // one thread per block of this workgroup's keys (whole blocks: T <= 256 / NQ)
+    if (tid < keys / T && row0 < ctx) {
+        float w = 0.f;
+        for (int t = tid * T / 32; t < (tid + 1) * T / 32; ++t) // 32-key tile t: group t / KT
+            for (int k = 0; k < NQ; ++k) w += s_sum[t / KT * NQ + k][t % KT];
+        float *dst = p.weights + (size_t)bh * p.nblk + (row0 >> p.t_shift);
+        *dst = row0 >= P ? w : *dst + w;
     }
 }
 
