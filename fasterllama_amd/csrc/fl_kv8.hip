@@ -83,8 +83,11 @@ void make_plan(const fl_attn_desc *d, int ctx, bool ragged, fl_attn_plan *plan)
 // Workspace: [arrivals B*H] [float output B*H*S*D] [part_o] [part_m] [part_l] [granules] [mask tile classes], and for the
 // block weights of a prompt [statistics B*H*S] [query operands] [query factors]; 256-byte sections.
 struct Layout {
-    size_t arrivals, tmp_out, part_o, part_m, part_l, granules, tile_class, stats, q_pairs, q_factor, total;
+    size_t arrivals, tmp_out, part_o, part_m, part_l, granules, tile_class, stats, q_pairs, q_factor, prompt_o, prompt_ml, total;
 };
+
+constexpr int kPromptWorkgroups = 512, kPromptMinTiles = 4;
+int partial_rows(int S) { return S < flattn::kPrefillQueriesPerBlock ? S : flattn::kPrefillQueriesPerBlock; }
 
 Layout layout(const fl_attn_desc *d, int S)
 {
@@ -105,8 +108,28 @@ Layout layout(const fl_attn_desc *d, int S)
     w.stats = take(bh * S32 * 8);
     w.q_pairs = take(D <= 128 ? bh * S32 * D * 4 : 0);
     w.q_factor = take(bh * S32 * 4);
+    // key splits of a prompt: at most kPromptWorkgroups partials (for this and for every shorter prompt) of up to 128 queries
+    const size_t rows = D <= 128 && bh * 2 <= kPromptWorkgroups ? kPromptWorkgroups * (size_t)partial_rows(S) : 0;
+    w.prompt_o = take(rows * D * 4);
+    w.prompt_ml = take(rows * 8);
     w.total = at;
     return w;
+}
+
+// Workgroups that share the keys of a (128-query block, head) of a prompt.  One workgroup walks its tiles at about 1 us each,
+// however few others there are, so a short piece behind a long context is bound by that walk; where the query blocks leave
+// the compute units' two workgroup slots empty, the keys are split, down to four tiles each, and a second launch merges.
+// Measured, whole call without / with the split, us (D = 128): 16 queries after 4000, 4 heads 166 / 36, 32 heads 171 / 39; 128 after
+// 1024, 8 heads 61 / 30; B=3, 5 heads (D = 96), 333 after 77 27.9 / 26.1; 512 queries, 32 heads 39.5 / 41.3.  Eight tiles
+// each are as good at 4000 rows and 2-4 us worse at 600-1500, two are 4-8 us worse; 1024 workgroups 55 at the second shape.
+int prompt_key_splits(const fl_attn_desc *d, int ctx, int S)
+{
+    if (d->size_per_head > 128) return 1;
+    const int64_t blocks = (int64_t)d->batch_size * d->head_num * ((S + flattn::kPrefillQueriesPerBlock - 1) / flattn::kPrefillQueriesPerBlock);
+    const int64_t tiles = (ctx + flattn::kPrefillKeysPerStep - 1) / flattn::kPrefillKeysPerStep;
+    int64_t n = kPromptWorkgroups / blocks;
+    if (n > tiles / kPromptMinTiles) n = tiles / kPromptMinTiles;
+    return (int)(n < 1 ? 1 : n);
 }
 
 int check_workspace(const void *ws, size_t bytes, const Layout &w)
@@ -193,10 +216,17 @@ hipError_t launch_prompt(const Kv8PromptParams &pp, hipStream_t stream)
             e = launch(flattn::prefill_mask_classify_kernel, dim3((unsigned)ktiles, qblocks), dim3(256), stream, pp.f, ktiles);
             if (e != hipSuccess) return e;
         }
-        const dim3 grid(qblocks * bh), block(256);
+        const dim3 grid(qblocks * bh * (unsigned)pp.key_splits), block(256);
         e = p.a.attn_mask ? launch(flattn::kv8_prefill_attn_kernel<D, true>, grid, block, stream, pp)
                           : launch(flattn::kv8_prefill_attn_kernel<D, false>, grid, block, stream, pp);
-        if (e != hipSuccess || !p.stats) return e;
+        if (e != hipSuccess) return e;
+        if (pp.key_splits > 1) {
+            const int64_t rows = (int64_t)bh * p.S;
+            constexpr int per = 256 / (D / 4);
+            e = launch(flattn::kv8_prompt_merge_kernel<D>, dim3((unsigned)((rows + per - 1) / per)), block, stream, pp);
+            if (e != hipSuccess) return e;
+        }
+        if (!p.stats) return e;
         // Query streams per workgroup of the block weights (see the kernel).  More streams, more and shorter workgroups, but each
         // reads the operands for fewer keys: split until there are four workgroups per compute unit (under a causal mask the
         // first keys' workgroups see every query, and with two per unit they finish last), not below four query blocks
@@ -383,6 +413,12 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
         pp.q_factor = reinterpret_cast<float *>(ws + w.q_factor);
         pp.first_block = (seq_len - p.weight_queries) / 32;
         pp.kept_blocks = (seq_len + 31) / 32 - pp.first_block;
+    }
+    pp.key_splits = prompt_key_splits(desc, io.start_pos + seq_len, seq_len);
+    if (pp.key_splits > 1) {
+        pp.part_o = reinterpret_cast<float *>(ws + w.prompt_o);
+        pp.part_ml = reinterpret_cast<float2 *>(ws + w.prompt_ml);
+        pp.part_rows = partial_rows(seq_len);
     }
     pp.k = p;
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);

@@ -289,7 +289,7 @@ __device__ __forceinline__ int kv8_splits(const Params &a, int T, int P) { retur
 // scores are formed, V's as soon as V is used up, so either half of a trip's arithmetic has the other matrix's loads in
 // flight, at no register's cost; the first trip is requested before the query has arrived.
 template <int D, bool HAS_MASK, bool PROMPT>
-__global__ __launch_bounds__(kKv8Waves * 64) __attribute__((amdgpu_waves_per_eu(3, 8)))
+__global__ __launch_bounds__(kKv8Waves * 64) __attribute__((amdgpu_waves_per_eu(D > 512 ? 2 : 3, 8)))
 void kv8_attn_kernel(const Kv8Params p)
 {
     typedef Kv8Geometry<D> G;

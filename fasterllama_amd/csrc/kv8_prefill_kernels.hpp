@@ -30,6 +30,10 @@ struct Kv8PromptParams {
     float *q_factor;      // [B*H, query blocks of 32, 32] with them
     int32_t first_block;  // 32-query blocks from here on are kept
     int32_t kept_blocks;
+    int32_t key_splits;   // workgroups that share the keys of a (query block, head); > 1: partials, merged by kv8_prompt_merge_kernel
+    int32_t part_rows;    // queries per partial: 128, or the prompt's where it is shorter
+    float *part_o;        // workspace [B*H * query blocks * splits, part_rows, D]: sums of weight * value, not normalised
+    float2 *part_ml;      // [.., part_rows]: (reference maximum, sum of weights)
 };
 
 // Four signed bytes as fp16: 1024 + (b ^ 128) is the fp16 with that low byte, minus 1152 leaves b, exactly.
@@ -87,7 +91,8 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     const PrefillParams &pf = pp.f;
     const int BH = a.B * a.H, S = p.S, P = a.start_pos, L = a.L;
     int qb, bh;
-    prefill_block_to_tile((int)blockIdx.x, BH, (S + kPrefillQueriesPerBlock - 1) / kPrefillQueriesPerBlock, HAS_MASK, qb, bh);
+    const int QB = (S + kPrefillQueriesPerBlock - 1) / kPrefillQueriesPerBlock, KS = pp.key_splits, split = (int)blockIdx.x / (QB * BH);
+    prefill_block_to_tile((int)blockIdx.x % (QB * BH), BH, QB, HAS_MASK, qb, bh);
     const int ctx = P + S, ctx8 = ctx & ~(p.T - 1); // rows [0, ctx8) are bytes, [ctx8, ctx) wait in the tail
     const int NT = (ctx + BN - 1) / BN;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -97,9 +102,16 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     auto build_list = [&](int c0, int c1, bool have_first, uint32_t w_first) __attribute__((always_inline)) -> int {
         return build_tile_list(pf, qb, c0, c1, NT, have_first, w_first, s_list, s_wave_cnt);
     };
+    // entry i of this workgroup's share, which starts at `share` of the pass's list
+    int share = 0;
     auto list_entry = [&](int c0, int i) __attribute__((always_inline)) -> uint32_t {
-        if constexpr (HAS_MASK) return s_list[i];
-        else return (uint32_t)(c0 + i) << 8 | 0x55u;
+        if constexpr (HAS_MASK) return s_list[share + i];
+        else return (uint32_t)(c0 + share + i) << 8 | 0x55u;
+    };
+    auto take_share = [&](int n) __attribute__((always_inline)) -> int { // of n listed tiles
+        if (KS == 1) return n;
+        share = (int)((int64_t)n * split / KS);
+        return (int)((int64_t)n * (split + 1) / KS) - share;
     };
 
     // global -> registers (fetch), registers -> LDS (commit) of a key tile.  A tile of the tail — fp16 rows, twice the loads, the
@@ -160,7 +172,7 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     };
 
     const int first_c1 = min(kTileListCap, NT);
-    fetch(0); // a guess at the first listed tile: right without a mask and under every causal one
+    if (split == 0) fetch(0); // a guess at the first listed tile: right without a mask and under every causal one
     uint32_t w_first = 0;
     if constexpr (HAS_MASK) {
         if (tid < first_c1) w_first = prompt_class_word(pf, qb, tid, NT);
@@ -288,7 +300,7 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
         const uint32_t e = qmax[qi] >> 23; // biased exponent of the largest element
         qc = a.scale * kLog2e * __uint_as_float((uint32_t)((int)e - 8) << 23);
         const int block = q_first / 32 - pp.first_block;
-        if (pp.q_pairs && block >= 0 && q_first < S) { // kept for the block weights
+        if (pp.q_pairs && split == 0 && block >= 0 && q_first < S) { // kept for the block weights
             half8 *dst = pp.q_pairs + ((size_t)bh * pp.kept_blocks + block) * (2 * NC * 64) + lane;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -301,9 +313,10 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     if constexpr (!HAS_MASK) __syncthreads(); // the slices lie in the tile buffers (with a mask the list's barriers see to it)
     int n_first = first_c1;
     if constexpr (HAS_MASK) n_first = build_list(0, first_c1, true, w_first);
+    n_first = take_share(n_first);
     if (n_first > 0) {
         const int t_first = (int)(__builtin_amdgcn_readfirstlane(list_entry(0, 0)) >> 8);
-        if (t_first != 0) fetch(t_first);
+        if (t_first != 0 || split != 0) fetch(t_first);
     }
 
     floatx16 ot[NDT];
@@ -320,9 +333,13 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     for (int c0 = 0; c0 < NT; c0 += kTileListCap) {
         const int c1 = min(c0 + kTileListCap, NT);
         int n = c1 - c0;
-        if (c0 == 0) n = n_first;
-        else if constexpr (HAS_MASK) n = build_list(c0, c1, false, 0u); // ends with a barrier
-        else __syncthreads();
+        if (c0 == 0) {
+            n = n_first;
+        } else {
+            if constexpr (HAS_MASK) n = build_list(c0, c1, false, 0u); // ends with a barrier
+            else __syncthreads();
+            n = take_share(n);
+        }
         if (n == 0) continue;
         uint32_t e0 = __builtin_amdgcn_readfirstlane(list_entry(c0, 0));
         uint32_t e1 = n > 1 ? __builtin_amdgcn_readfirstlane(list_entry(c0, 1)) : 0u;
@@ -466,13 +483,17 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     }
 
     l += __shfl_xor(l, 32);
-    if (p.stats && hf == 0 && q_row < S) p.stats[(size_t)bh * S + q_row] = make_float2(m, l);
+    const size_t slot = ((size_t)bh * QB + qb) * KS + split; // of the partials
+    if (hf == 0 && q_row < S) {
+        if (KS > 1) pp.part_ml[slot * pp.part_rows + wave * 32 + qi] = make_float2(m, l);
+        else if (p.stats) p.stats[(size_t)bh * S + q_row] = make_float2(m, l);
+    }
     // e^(..) sums to l, accumulators are in units of vref with weights times 2^7; a fully masked query: 0 / 0
-    const float rl = __uint_as_float(vref) * (1.0f / 128.0f) / l;
+    const float rl = __uint_as_float(vref) * (1.0f / 128.0f) / (KS > 1 ? 1.0f : l);
     __syncthreads(); // every wave is done with the last tile
     float *so = reinterpret_cast<float *>(smem) + wave * 32 * LDO;
     const int q0 = qb * kPrefillQueriesPerBlock + wave * 32;
-    float *dst0 = a.out + ((size_t)bh * S + q0) * D;
+    float *dst0 = KS > 1 ? pp.part_o + (slot * pp.part_rows + wave * 32) * D : a.out + ((size_t)bh * S + q0) * D;
     constexpr int LPRW = HALF_D / 4, ROWS = 64 / LPRW;
 #pragma unroll
     for (int pass = 0; pass < D / HALF_D; ++pass) {
@@ -493,6 +514,36 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
         }
         wave_lds_sync(); // the slice is rewritten by the next pass
     }
+}
+
+// Merges the key splits of every query: out = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(m_s - max m).  D/4 lanes per query;
+// grid = ceil(B*H*S / (1024 / D)), block = 256.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_prompt_merge_kernel(const Kv8PromptParams pp)
+{
+    constexpr int TPR = D / 4, ROWS = 256 / TPR; // (size_per_head 96: the last 16 threads own no query)
+    const Kv8Params &p = pp.k;
+    const int S = p.S, QB = (S + kPrefillQueriesPerBlock - 1) / kPrefillQueriesPerBlock, KS = pp.key_splits;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+    if (threadIdx.x >= ROWS * TPR || row >= (int64_t)p.a.B * p.a.H * S) return;
+    const int bh = (int)(row / S), q = (int)(row % S), t = threadIdx.x % TPR;
+    const size_t slot0 = ((size_t)bh * QB + q / kPrefillQueriesPerBlock) * KS, at = q % kPrefillQueriesPerBlock;
+    float M = kMaxFloor * kLog2e;
+    for (int s = 0; s < KS; ++s) M = fmaxf(M, pp.part_ml[(slot0 + s) * pp.part_rows + at].x);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < KS; ++s) {
+        const size_t i = (slot0 + s) * pp.part_rows + at;
+        const float2 ml = pp.part_ml[i];
+        const float4 x = reinterpret_cast<const float4 *>(pp.part_o + i * D)[t];
+        const float w = __builtin_amdgcn_exp2f(ml.x - M);
+        l = fmaf(ml.y, w, l);
+        o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
+    }
+    o.x /= l; o.y /= l; o.z /= l; o.w /= l;
+    reinterpret_cast<float4 *>(p.a.out + (size_t)row * D)[t] = o;
+    if (p.stats && t == 0) p.stats[row] = make_float2(M, l);
 }
 
 // Block weights of a prompt: weights[b,h,blk] (+)= sum over the last weight_queries queries and the block's rows of

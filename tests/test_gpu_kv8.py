@@ -293,6 +293,32 @@ def test_prompt_scores_of_every_size(gpu):
     assert_cache(c.gpu, c.ref, 400, 400)
 
 
+@pytest.mark.parametrize("D,T,dtype", [(128, 64, "f16"), (96, 32, "f32"), (32, 128, "f16")])
+@pytest.mark.parametrize("kind", [None, "causal", "inf_window", "strict"])
+def test_prompt_pieces_behind_a_long_context_share_their_keys(gpu, D, T, dtype, kind):
+    """Few queries, many keys: the keys are split over workgroups, some of which a window leaves nothing."""
+    for start, S in ((1301, 3), (1100, 130), (0, 1)):
+        c = Case(gpu, 1, 2, D, 1536, T, dtype, start, weights=True, max_seq_len=200)
+        got, want, tol = c.prompt(S, masks(kind, 1536), weight_queries=2)
+        assert_out(got, want, tol, f"start {start} S {S}")
+        assert_cache(c.gpu, c.ref, S, start + S)
+
+
+def test_non_finite_prompt_inputs_do_not_spread(gpu):
+    c = Case(gpu, 1, 2, 64, 256, 32, "f32", 0, max_seq_len=100)
+    raw, val, _ = c.feed(100, 3)
+    q, k, v = (x.copy() for x in val)
+    k[0, 3, 0, 5], k[0, 40, 1, 6], v[0, 99, 0, 7], v[0, 70, 1, 8], v[0, 2, 1, 0] = np.nan, np.inf, -np.inf, 1e30, np.nan
+    q[0, 50, 1, 3], q[0, 51, 0, 0] = np.nan, np.inf
+    m = masks("causal", 256)
+    got = c.op.prefill(c.t(q), c.t(k), c.t(v), c.gpu, c.table_d, attn_mask=c.t(m))
+    with np.errstate(invalid="ignore"):
+        want, tol = c.ref.step(q, k, v, c.table, c.rows, m)
+    assert np.isnan(want[0, 1, 50]).all() and np.isnan(want[0, 0, 51]).all()
+    assert_out(got[:, [0]], want[:, [0]], tol)  # (head 1's 65504 is a scale of its own)
+    assert_cache(c.gpu, c.ref, 100, 100)
+
+
 def test_prompt_with_a_persistent_class_table_and_int8_output(gpu):
     import torch
     from fasterllama_amd.decode_attn import PrefillAttention

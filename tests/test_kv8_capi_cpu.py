@@ -160,6 +160,12 @@ def test_cache_bytes_and_workspace_sizes():
         assert lib.fl_kv8_workspace_bytes(C.byref(d), 32, 1, C.byref(n)) == 0
         assert lib.fl_kv8_workspace_bytes(C.byref(d), 32, 500, C.byref(m)) == 0
         assert n.value % 256 == 0 and m.value >= n.value >= 8 * (4 + D * 4 + 7 * (D + 2) * 4 + 1024 // 32 * 8)
+    # a workspace for prompts of up to S tokens serves every shorter one
+    for B, H, D in ((1, 4, 128), (3, 43, 96), (1, 129, 32), (2, 128, 64), (1, 257, 128), (1, 8, 256)):
+        d, last = desc(B=B, H=H, D=D, L=1024), 0
+        for S in (1, 2, 31, 32, 33, 127, 128, 129, 256, 257, 512, 1024):
+            assert lib.fl_kv8_workspace_bytes(C.byref(d), 64, S, C.byref(n)) == 0 and n.value >= last
+            last = n.value
     assert lib.fl_kv8_workspace_bytes(C.byref(desc()), 64, 1, None) == capi.FL_ATTN_ERR_NULL_POINTER
 
 
