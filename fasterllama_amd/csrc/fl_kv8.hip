@@ -316,7 +316,8 @@ int fl_kv8_workspace_init(const fl_attn_desc *desc, int32_t block_len, int32_t s
     return FL_ATTN_OK;
 }
 
-int fl_kv8_decode_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io_in, const int32_t *rope_row_per_seq, void *hip_stream)
+int fl_kv8_decode_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io_in, const int32_t *rope_row_per_seq, int32_t rope_table_rows,
+                          void *hip_stream)
 {
     fl_attn_desc desc_copy;
     int st = import_desc(&desc, &desc_copy);
@@ -331,6 +332,7 @@ int fl_kv8_decode_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, c
     if (st != FL_ATTN_OK) return st;
     if ((io.flags & ~FL_ATTN_IO_WORKSPACE_READY) != 0) return FL_ATTN_ERR_ARGUMENT;
     if ((reinterpret_cast<uintptr_t>(rope_row_per_seq) & 3u) != 0) return FL_ATTN_ERR_ALIGNMENT;
+    if (rope_row_per_seq && rope_table_rows < 1) return FL_ATTN_ERR_POSITION;
     const int L = desc->total_len, D = desc->size_per_head;
     const bool ragged = io.start_pos_per_seq != nullptr;
     int max_pos = io.start_pos;
@@ -352,6 +354,7 @@ int fl_kv8_decode_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, c
     Kv8Params p = make_params(desc, &c, &io);
     p.a.pos_per_seq = io.start_pos_per_seq;
     p.rope_rows = rope_row_per_seq;
+    p.table_rows = rope_table_rows;
     p.a.out = io.out ? io.out : reinterpret_cast<float *>(ws + w.tmp_out);
     p.a.max_pos = max_pos; p.a.chunk = plan.chunk_rows; p.a.split_cap = cap; p.a.direct = direct;
     if (!direct) {
@@ -388,7 +391,9 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
     if (seq_len < 1 || io.start_pos < 0 || (int64_t)io.start_pos + seq_len > L) return FL_ATTN_ERR_POSITION;
     if (io.attn_mask && (io.mask_ld < 0 || (io.mask_ld != 0 && io.mask_ld < (int64_t)io.start_pos + seq_len))) return FL_ATTN_ERR_ARGUMENT;
     if (c.weights && D > 128) return FL_ATTN_ERR_HEAD_DIM;
-    if ((int64_t)desc->batch_size * desc->head_num * seq_len > (int64_t)INT32_MAX) return FL_ATTN_ERR_SHAPE; // a workgroup per query and head
+    // a workgroup per query and head where the head size is beyond 128; the mask's classes are a two-dimensional grid
+    if ((int64_t)desc->batch_size * desc->head_num * seq_len > (int64_t)INT32_MAX || seq_len > 65535 * flattn::kPrefillQueriesPerBlock)
+        return FL_ATTN_ERR_SHAPE;
     const Layout w = layout(desc, seq_len);
     st = check_workspace(io.workspace, io.workspace_bytes, w);
     if (st != FL_ATTN_OK) return st;

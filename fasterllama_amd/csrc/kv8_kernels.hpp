@@ -30,6 +30,7 @@ struct Kv8Params {
     float *weights;           // [B*H, nblk] accumulated softmax weight, or NULL
     float2 *granules;         // workspace [B*H, L / granule rows]: (reference maximum, sum of weights) of a few rows
     const int32_t *rope_rows; // [B] table rows, or NULL: a.rope_row
+    int32_t table_rows;       // rows of the table, where rope_rows is given
     int32_t in_kind;
     int32_t T, t_shift;       // rows per block, log2
     int32_t nblk;             // L / T
@@ -270,6 +271,13 @@ __device__ __forceinline__ void quantise_tail(const _Float16 *tail, int8_t *rows
     if (tid == 0) *scale_at = absmax / 127.0f;
 }
 
+// Whether sequence b's device-side position lies in the cache and the plan, and its table row in the table.
+__device__ __forceinline__ bool kv8_position_ok(const Kv8Params &p, int b, int P)
+{
+    if (P < 0 || P >= p.a.L || P > p.a.max_pos) return false;
+    return !p.rope_rows || (uint32_t)p.rope_rows[b] < (uint32_t)p.table_rows;
+}
+
 // Splits of one (b,h) in a decode step whose context is split: `chunk` rows of the complete blocks each, and one more for the
 // newest row and the open block's rows before it (or for the block that the newest row completes).
 __device__ __forceinline__ int kv8_splits(const Params &a, int T, int P) { return (P - (P & (T - 1)) + a.chunk - 1) / a.chunk + 1; }
@@ -321,7 +329,7 @@ void kv8_attn_kernel(const Kv8Params p)
         b = bh / H;
         h = bh % H;
         P = a.pos_per_seq ? a.pos_per_seq[b] : a.start_pos;
-        if (P < 0 || P >= L || P > a.max_pos) { // outside the cache or the plan: store nothing, poison the output
+        if (!kv8_position_ok(p, b, P)) { // store nothing, poison the output
             if ((a.direct || a.arrivals) && split == 0)
                 for (int d = tid; d < D; d += kKv8Waves * 64) a.out[(size_t)bh * D + d] = __builtin_nanf("");
             return;
@@ -749,7 +757,7 @@ __global__ __launch_bounds__(kCombineThreads) void kv8_combine_kernel(const Kv8P
     __shared__ CombineShared<D> sh;
     const int bh = blockIdx.x, tid = threadIdx.x, b = bh / p.a.H;
     const int P = p.a.pos_per_seq ? p.a.pos_per_seq[b] : p.a.start_pos;
-    if (P < 0 || P >= p.a.L || P > p.a.max_pos) {
+    if (!kv8_position_ok(p, b, P)) {
         for (int d = tid; d < D; d += kCombineThreads) p.a.out[(size_t)bh * D + d] = __builtin_nanf("");
         return;
     }

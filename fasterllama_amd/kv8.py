@@ -172,7 +172,7 @@ class KV8Attention:
         B, H, L, D = self.shape
         self._cache(cache)
         last = start_pos if start_pos_per_seq is None else (L - 1 if max_start_pos < 0 else max_start_pos)
-        # (rows named on the device cannot be looked at here)
+        # (rows named on the device are looked at there)
         rope_rows = 0 if rope_row_per_seq is not None else (last if rope_row < 0 else rope_row) + 1
         out = self._fill(q, k_new, v_new, 1, freq_cis, rope_rows, attn_mask, last, scales, out, (B, H * D), out_int8, out_scale)
         io = self.io
@@ -180,7 +180,7 @@ class KV8Attention:
         io.start_pos, io.max_start_pos, io.rope_row = start_pos, max_start_pos, rope_row
         io.flags = capi.FL_ATTN_IO_WORKSPACE_READY
         self._enqueue(self.lib.fl_kv8_decode_forward, self._desc, cache.ref, self._io,
-                      self._vector("rope_row_per_seq", rope_row_per_seq, torch.int32, B))
+                      self._vector("rope_row_per_seq", rope_row_per_seq, torch.int32, B), freq_cis.shape[0])
         return out
 
     def prefill(self, q, k_new, v_new, cache: KV8Cache, freq_cis, start_pos: int = 0, attn_mask=None, mask_tile_classes=None,
@@ -198,7 +198,11 @@ class KV8Attention:
         io = self.io
         io.start_pos_per_seq = None
         io.start_pos, io.max_start_pos, io.rope_row, io.flags = start_pos, -1, rope_row, 0
-        io.mask_tile_classes = None if mask_tile_classes is None else mask_tile_classes.data_ptr()
+        if mask_tile_classes is None:
+            io.mask_tile_classes = None
+        else:
+            n = -(-L // 32)
+            io.mask_tile_classes = self._vector("mask_tile_classes", mask_tile_classes, torch.uint8, n * -(-n // 4) * 4)
         self._enqueue(self.lib.fl_kv8_prefill_forward, self._desc, cache.ref, self._io, S, weight_queries)
         return out
 

@@ -265,9 +265,11 @@ int fl_kv8_workspace_init(const fl_attn_desc *desc, int32_t block_len, int32_t s
                           size_t workspace_bytes, void *hip_stream);
 
 /* One decode step: RoPE, append, attention over rows [0, start_pos].  rope_row_per_seq: NULL, or [B] table rows on the
- * device in place of io.rope_row — after an eviction a sequence's next row is not its position. */
+ * device in place of io.rope_row — after an eviction a sequence's next row is not its position.  freq_cis then has
+ * rope_table_rows rows (ignored otherwise), and a sequence whose entry lies outside them is treated like one whose
+ * position lies outside the cache: NaN output, nothing stored. */
 int fl_kv8_decode_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io,
-                          const int32_t *rope_row_per_seq, void *hip_stream);
+                          const int32_t *rope_row_per_seq, int32_t rope_table_rows, void *hip_stream);
 
 /* The prompt phase (layouts and mask as fl_prefill_attn_forward).  With cache.weights, the last weight_queries queries
  * of every sequence add theirs (0 = all); served for size_per_head <= 128 (FL_ATTN_ERR_HEAD_DIM). */
@@ -289,7 +291,8 @@ typedef struct fl_kv8_evict_args {
     int32_t rows;                /* rows in the cache (= the next start_pos) */
     const int32_t *rows_per_seq; /* NULL, or [B] on the device; a count outside [0, L] moves nothing: kept and
                                     rows_out are -1 for that sequence */
-    int32_t keep_blocks;         /* >= 1, at most to_total_len / block_len */
+    int32_t keep_blocks;         /* >= 1, at most to_total_len / block_len; a smaller number leaves the open block a
+                                    place (without one, rows_out passes to_total_len and the next step is refused) */
     int32_t recent_blocks;       /* 0 .. keep_blocks */
     int32_t to_total_len;        /* rows per (b,h) of `to`; 0 = desc.total_len */
     int32_t reserved;            /* 0 */

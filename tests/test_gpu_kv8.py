@@ -191,6 +191,72 @@ def test_decode_ragged_with_positions_outside(gpu, dtype, nsplit):
     assert_cache(c.gpu, c.ref)
 
 
+def test_table_rows_outside_the_table_store_nothing(gpu):
+    for nsplit in (1, 3):
+        c = Case(gpu, 4, 2, 64, 640, 32, "f16", [500, 501, 502, 503], weights=True, nsplit=nsplit)
+        before = c.ref.copy()
+        raw, val, _ = c.feed(1, 7)
+        rope = np.array([704, 703, -1, 2 ** 31 - 1])  # the table has 704 rows
+        got = c.op.decode(*raw, c.gpu, c.table_d, start_pos_per_seq=c.t(c.rows.astype(np.int32)), max_start_pos=503, rope_row_per_seq=c.t(rope.astype(np.int32)))
+        want, tol = c.ref.step(*val, c.table, [-1, 501, -1, -1], rope=rope)
+        assert_out(got, want[:, :, 0], tol[..., 0])
+        assert_cache(c.gpu, c.ref)
+
+
+def test_two_objects_on_two_streams(gpu):
+    """Each has its workspace: split steps side by side."""
+    import torch
+    cases = [Case(gpu, 1, 8, 128, 4096, 64, "f16", 4000 + 63 * i, weights=True, seed=i) for i in range(2)]
+    streams = [torch.cuda.Stream(gpu) for _ in cases]
+    torch.cuda.synchronize()
+    feeds = [c.feed(1, 5) for c in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, s, (raw, _, _) in zip(cases, streams, feeds):
+            with torch.cuda.stream(s):
+                c.gpu.weights.zero_()
+                c.got = c.op.decode(*raw, c.gpu, c.table_d, start_pos=int(c.rows[0]))
+    torch.cuda.synchronize()
+    for c, (_, val, _) in zip(cases, feeds):
+        c.ref.weights[:] = 0
+        want, tol = c.ref.step(*val, c.table, c.rows)
+        assert_out(c.got, want[:, :, 0], tol[..., 0])
+        assert_cache(c.gpu, c.ref)
+
+
+def test_wrapper_refusals(gpu):
+    import torch
+    c = Case(gpu, 2, 2, 64, 128, 32, "f16", 5, weights=True, max_seq_len=16)
+    (q, k, v), _, _ = c.feed(1, 1)
+    bad = [dict(q=q.float()), dict(q=q[:, :, :1]), dict(q=q.transpose(2, 3)), dict(q=q.cpu()), dict(freq=c.table_d[:4]), dict(freq=c.table_d[:, :32]),
+           dict(attn_mask=torch.zeros(3, 128, device=gpu)), dict(attn_mask=torch.zeros(128, 5, device=gpu)), dict(attn_mask=torch.zeros(128, 128, device=gpu).t()),
+           dict(start_pos=128), dict(start_pos=-1), dict(start_pos_per_seq=torch.zeros(3, dtype=torch.int32, device=gpu)),
+           dict(start_pos_per_seq=torch.zeros(2, dtype=torch.int64, device=gpu)), dict(out=torch.empty(2, 64, device=gpu)),
+           dict(cache=to_gpu(kr.Cache(2, 2, 64, 160, 32), gpu)), dict(cache=to_gpu(kr.Cache(2, 2, 64, 128, 64), gpu))]
+    for kw in bad:
+        a = {"q": q, "cache": c.gpu, "freq": c.table_d, "start_pos": 5, **kw}
+        rest = {n: x for n, x in a.items() if n not in ("q", "cache", "freq")}
+        with pytest.raises(capi.FlAttnError):
+            c.op.decode(a["q"], k, v, a["cache"], a["freq"], **rest)
+    (q, k, v), _, _ = c.feed(17, 1)
+    with pytest.raises(capi.FlAttnError):
+        c.op.prefill(q, k, v, c.gpu, c.table_d)
+    (q, k, v), _, _ = c.feed(16, 1)
+    with pytest.raises(capi.FlAttnError):
+        c.op.prefill(q, k, v, c.gpu, c.table_d, start_pos=113)
+    with pytest.raises(capi.FlAttnError):
+        c.op.prefill(q, k, v, c.gpu, c.table_d, mask_tile_classes=torch.zeros(7, dtype=torch.uint8, device=gpu))
+    for rows in (0, 129):
+        with pytest.raises(capi.FlAttnError):
+            c.op.read(c.gpu, rows)
+    for keep, recent, rows in ((0, 0, 64), (5, 0, 64), (2, 3, 64), (2, 1, 129)):
+        with pytest.raises(capi.FlAttnError):
+            c.op.evict(c.gpu, keep, recent, rows)
+    with pytest.raises(capi.FlAttnError):
+        c.op.evict(to_gpu(kr.Cache(2, 2, 64, 128, 32), gpu), 1, 0, 64)
+    torch.cuda.synchronize()
+
+
 def test_decode_scales_of_stale_blocks_and_rows_are_never_read(gpu):
     """The whole cache behind the rows is NaN scales and random integers (Cache's junk): the last trip of a wave reaches over
     the last complete block at head sizes whose trips are longer than a block."""

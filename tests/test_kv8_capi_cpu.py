@@ -34,8 +34,8 @@ def fake_io(**over):
     return io
 
 
-def decode(d=None, c=None, io=None, rope=None):
-    return capi.load().fl_kv8_decode_forward(C.byref(d or desc()), C.byref(c or fake_cache()), C.byref(io or fake_io()), rope, None)
+def decode(d=None, c=None, io=None, rope=None, rows=64):
+    return capi.load().fl_kv8_decode_forward(C.byref(d or desc()), C.byref(c or fake_cache()), C.byref(io or fake_io()), rope, rows, None)
 
 
 def prefill(d=None, c=None, io=None, S=8, W=0):
@@ -102,6 +102,7 @@ def test_io(over, want):
 
 def test_decode_only_and_prompt_only():
     assert decode(rope=0x1002) == capi.FL_ATTN_ERR_ALIGNMENT
+    assert decode(rope=0x1000, rows=0) == capi.FL_ATTN_ERR_POSITION
     assert decode(io=fake_io(start_pos_per_seq=0x1000, max_start_pos=256)) == capi.FL_ATTN_ERR_POSITION
     assert prefill(io=fake_io(start_pos_per_seq=0x1000)) == capi.FL_ATTN_ERR_ARGUMENT
     assert prefill(S=0) == capi.FL_ATTN_ERR_POSITION and prefill(S=254) == capi.FL_ATTN_ERR_POSITION
