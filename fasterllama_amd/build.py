@@ -19,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -184,17 +185,21 @@ def build_cxxbench() -> str:
 def run_sanitizers() -> None:
     """Host code under AddressSanitizer + UndefinedBehaviorSanitizer, built and RUN here (no GPU involved):
     the CPU oracle with its driver (`make -C oracle asan`), and the host pass of the C-ABI library with
-    tests/cpp/capi_host_check.cpp (validation, planning and workspace arithmetic; every call is rejected
-    before a launch).  Raises when a sanitizer reports or a check fails."""
+    tests/cpp/capi_host_check.cpp and kv8_host_check.cpp (validation, planning and workspace arithmetic; every call
+    is rejected before a launch).  Raises when a sanitizer reports or a check fails."""
     _run(["make", "-C", os.path.join(ROOT, "oracle"), "-B", "asan"])
-    exe = os.path.join(ROOT, "tests", "cpp", "capi_host_check")
-    _run([hipcc(), f"--offload-arch={GFX_ARCH}", "-O1", "-g", "-std=c++17",
-          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unknown-warning-option",
-          "-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
-          "-Xarch_host", "-fno-sanitize-recover=all",
-          "-I", os.path.join(ROOT, "include"), "-o", exe,
-          *(os.path.join(CSRC, f) for f in HIP_SOURCES), os.path.join(ROOT, "tests", "cpp", "capi_host_check.cpp")])
-    _run([exe])
+    flags = [f"--offload-arch={GFX_ARCH}", "-O1", "-g", "-std=c++17",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unknown-warning-option",
+             "-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
+             "-Xarch_host", "-fno-sanitize-recover=all"]
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, f.replace(".hip", ".o")) for f in HIP_SOURCES]
+        with ThreadPoolExecutor() as pool:
+            list(pool.map(lambda so: _run([hipcc(), *flags, "-c", "-o", so[1], os.path.join(CSRC, so[0])]), zip(HIP_SOURCES, objects)))
+        for name in ("capi_host_check", "kv8_host_check"):
+            exe = os.path.join(ROOT, "tests", "cpp", name)
+            _run([hipcc(), *flags, "-I", os.path.join(ROOT, "include"), "-o", exe, *objects, exe + ".cpp"])
+            _run([exe])
 
 
 TARGETS = {
