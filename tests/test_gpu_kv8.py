@@ -370,6 +370,66 @@ def test_prompt_pieces_behind_a_long_context_share_their_keys(gpu, D, T, dtype, 
         assert_cache(c.gpu, c.ref, S, start + S)
 
 
+@pytest.mark.parametrize("kind", [None, "padding"])
+def test_prompt_over_more_tiles_than_one_list(gpu, kind):
+    """33 100 keys: the tile list is built twice."""
+    import torch
+    c = Case(gpu, 1, 1, 32, 128 * 259, 128, "f16", 0, max_seq_len=64, weights=True)
+    r = np.random.RandomState(0)
+    n, start, S = 128 * 259, 33060, 40
+    c.ref.k_scale[:], c.ref.v_scale[:], c.ref.weights[:] = 0.01 + 0.02 * r.rand(1, 1, 259), 0.01 + 0.02 * r.rand(1, 1, 259), 0
+    c.ref.k_tail[:], c.ref.v_tail[:] = r.randn(1, 1, 128, 32), r.randn(1, 1, 128, 32)
+    c.gpu, c.rows = to_gpu(c.ref, gpu), np.array([start])
+    raw, val, _ = c.feed(S, 5)
+    m = None
+    if kind:
+        m = np.zeros((1, n), np.float32)
+        m[0, :1000], m[0, 20000:30000] = NEG, -np.inf
+    got = c.op.prefill(*raw, c.gpu, c.table_d, start_pos=start, attn_mask=c.t(m), weight_queries=7)
+    want, tol = c.ref.step(*val, c.table, [start], None if m is None else np.broadcast_to(m, (n, n)), weight_queries=7)
+    assert_out(got, want, tol)
+    assert_cache(c.gpu, c.ref, S, start + S)
+
+
+def test_graph_of_a_prompt_an_eviction_and_a_read(gpu):
+    """Captured once, replayed with eager work between: every replay equals the eager run."""
+    import torch
+    c = Case(gpu, 2, 4, 128, 512, 64, "f16", 70, weights=True, max_seq_len=300)
+    m = c.t(masks("causal", 512))
+    raw, _, _ = c.feed(300, 3)
+    start = to_gpu(c.ref, gpu)
+    names = c.ref.names()
+
+    def restore():
+        for n in names:
+            getattr(c.gpu, n).copy_(getattr(start, n))
+
+    def run():
+        out = c.op.prefill(*raw, c.gpu, c.table_d, start_pos=70, attn_mask=m, weight_queries=100)
+        kept, rows = c.op.evict(c.gpu, 3, 1, 370)
+        return (out, kept, rows, *c.op.read(c.gpu, 3 * 64 + 370 % 64))
+    side = torch.cuda.Stream(gpu)
+    side.wait_stream(torch.cuda.current_stream(gpu))
+    with torch.cuda.stream(side):
+        want = [x.clone() for x in run()]
+        state = {n: getattr(c.gpu, n).clone() for n in names}
+    torch.cuda.synchronize()
+    restore()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run()
+    for _ in range(4):
+        restore()
+        for x in got:
+            x.fill_(3)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        for n in names:
+            assert torch.equal(getattr(c.gpu, n).float().nan_to_num(7.0), state[n].float().nan_to_num(7.0)), n
+
+
 def test_non_finite_prompt_inputs_do_not_spread(gpu):
     c = Case(gpu, 1, 2, 64, 256, 32, "f32", 0, max_seq_len=100)
     raw, val, _ = c.feed(100, 3)
