@@ -391,8 +391,11 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
     if (seq_len < 1 || io.start_pos < 0 || (int64_t)io.start_pos + seq_len > L) return FL_ATTN_ERR_POSITION;
     if (io.attn_mask && (io.mask_ld < 0 || (io.mask_ld != 0 && io.mask_ld < (int64_t)io.start_pos + seq_len))) return FL_ATTN_ERR_ARGUMENT;
     if (c.weights && D > 128) return FL_ATTN_ERR_HEAD_DIM;
-    // a workgroup per query and head where the head size is beyond 128; the mask's classes are a two-dimensional grid
-    if ((int64_t)desc->batch_size * desc->head_num * seq_len > (int64_t)INT32_MAX || seq_len > 65535 * flattn::kPrefillQueriesPerBlock)
+    // A workgroup per query and head where the head size is beyond 128, of the 2^32 threads a launch may have; the mask's
+    // classes are a two-dimensional grid.
+    const int64_t queries = (int64_t)desc->batch_size * desc->head_num * seq_len;
+    if (queries > (int64_t)INT32_MAX || (D > 128 && queries * flattn::kKv8Waves * 64 > (int64_t)UINT32_MAX) ||
+        seq_len > 65535 * flattn::kPrefillQueriesPerBlock)
         return FL_ATTN_ERR_SHAPE;
     const Layout w = layout(desc, seq_len);
     st = check_workspace(io.workspace, io.workspace_bytes, w);
@@ -449,7 +452,7 @@ int fl_kv8_read(const fl_attn_desc *desc, const fl_kv8_cache *cache, int32_t row
     p.a.pos_per_seq = rows_per_seq;
     const int D = desc->size_per_head, vec = desc->dtype == FL_ATTN_F16 ? 8 : 4;
     const int64_t groups = ((int64_t)rows * (D / vec) + 1023) / 1024, grid = groups * 2 * desc->batch_size * desc->head_num;
-    if (grid > INT32_MAX) return FL_ATTN_ERR_SHAPE;
+    if (grid > INT32_MAX / 128) return FL_ATTN_ERR_SHAPE; // 2^32 threads a launch
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     const hipError_t e = desc->dtype == FL_ATTN_F16
                              ? launch(flattn::kv8_read_kernel<_Float16>, dim3((unsigned)grid), dim3(256), stream, p, static_cast<_Float16 *>(k_out),
@@ -480,6 +483,11 @@ int fl_kv8_evict(const fl_attn_desc *desc, const fl_kv8_cache *from, const fl_kv
     if (!s.weights || !t.weights || !args.kept || !args.rows_out) return FL_ATTN_ERR_NULL_POINTER;
     for (const void *f : {(const void *)args.kept, (const void *)args.rows_out, (const void *)args.rows_per_seq})
         if ((reinterpret_cast<uintptr_t>(f) & 3u) != 0) return FL_ATTN_ERR_ALIGNMENT;
+    // one workgroup writes rows_out while others still read rows_per_seq
+    const size_t counts = (size_t)desc->batch_size * 4, listed = counts * desc->head_num * (size_t)(args.keep_blocks > 0 ? args.keep_blocks : 1);
+    if (overlap(args.kept, listed, args.rows_out, counts) ||
+        (args.rows_per_seq && (overlap(args.rows_per_seq, counts, args.rows_out, counts) || overlap(args.rows_per_seq, counts, args.kept, listed))))
+        return FL_ATTN_ERR_ARGUMENT;
     if (s.block_len != t.block_len) return FL_ATTN_ERR_ARGUMENT;
     const int T = s.block_len, L = desc->total_len, L_to = desc_to.total_len, D = desc->size_per_head;
     if (!args.rows_per_seq && (args.rows < 0 || args.rows > L)) return FL_ATTN_ERR_POSITION;
@@ -512,7 +520,7 @@ int fl_kv8_evict(const fl_attn_desc *desc, const fl_kv8_cache *from, const fl_kv
     p.nblk = L / T; p.nblk_to = L_to / T; p.keep = args.keep_blocks; p.recent = args.recent_blocks;
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
     const int slices = (T * D / 16 + 255) / 256;
-    if ((int64_t)bh * 2 * slices > INT32_MAX) return FL_ATTN_ERR_SHAPE;
+    if ((int64_t)bh * 2 * slices > INT32_MAX / 128) return FL_ATTN_ERR_SHAPE;
     if (!check_hip(launch(flattn::kv8_select_kernel, dim3((unsigned)bh), dim3(256), stream, p))) return FL_ATTN_ERR_HIP;
     if (!check_hip(launch(flattn::kv8_move_kernel, dim3((unsigned)(bh * 2 * slices)), dim3(256), stream, p, slices))) return FL_ATTN_ERR_HIP;
     return FL_ATTN_OK;

@@ -216,8 +216,11 @@ template <int D, typename LOAD>
 __device__ __forceinline__ void add_block_weights(const Kv8Params &p, int bh, int P, float M, float Lsum, int tid, LOAD granule, float old)
 {
     constexpr int GR = Kv8Geometry<D>::GR;
-    if (!(Lsum > 0.f)) return; // every key masked: the output is NaN, nothing was attended to
     const int blk_new = P >> p.t_shift;
+    if (!(Lsum > 0.f)) { // every key masked: the output is NaN, nothing was attended to
+        if (tid == 0 && (P & (p.T - 1)) == 0) p.weights[(size_t)bh * p.nblk + blk_new] = 0.f;
+        return;
+    }
     const bool open = ((P + 1) & (p.T - 1)) != 0; // the last block's rows are in the tail: one granule for all of them
     const int per = p.T / GR;
     const float rl = 1.0f / Lsum;
@@ -943,8 +946,8 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Params p, O *out
     typedef O vec __attribute__((ext_vector_type(VEC)));
     const int bh = blockIdx.x / groups >> 1, b = bh / p.a.H;
     const bool is_v = (blockIdx.x / groups & 1) != 0;
-    int rows = p.a.pos_per_seq ? p.a.pos_per_seq[b] : n;
-    rows = min(rows, min(n, p.a.L)); // (a negative count: all zeros)
+    // rows in the cache (a negative count: all zeros): where they end, not where the output does, the tail begins
+    const int rows = min(p.a.pos_per_seq ? p.a.pos_per_seq[b] : n, p.a.L);
     const int rows8 = rows > 0 ? rows & ~(p.T - 1) : 0;
     const int8_t *src = (is_v ? p.v8 : p.k8) + (size_t)bh * p.a.L * D;
     const _Float16 *tail = (is_v ? p.v_tail : p.k_tail) + (size_t)bh * p.T * D;

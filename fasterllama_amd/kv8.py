@@ -68,8 +68,8 @@ class KV8Cache:
 
 
 class KV8Attention:
-    """Attention over caller-owned KV8Caches of one shape, with a workspace of its own: calls of one object go to one stream at
-    a time.  dtype is the type of q, k_new, v_new (float32 or float16) and of what read() returns."""
+    """Attention over caller-owned KV8Caches of one shape, with a workspace of its own: calls of one object come from one thread
+    and go to one stream at a time.  dtype is the type of q, k_new, v_new (float32 or float16) and of what read() returns."""
 
     def __init__(self, batch_size: int, head_num: int, size_per_head: int, total_len: int, dtype: torch.dtype = torch.float16,
                  block_len: int = 64, max_seq_len: int = 1, nsplit: int = 0, softmax_scale: float = 0.0,
@@ -207,7 +207,8 @@ class KV8Attention:
         return out
 
     def read(self, cache: KV8Cache, rows: int, rows_per_seq=None):
-        """The values of rows [0, rows): k, v [B,H,rows,D] in dtype; zeros from rows_per_seq[b] (int32 [B]) on."""
+        """The values of rows [0, rows): k, v [B,H,rows,D] in dtype.  rows: of every sequence, or rows_per_seq int32 [B], how
+        many each holds; zeros from there on."""
         B, H, _, D = self.shape
         self._cache(cache)
         k = torch.empty(B, H, max(rows, 0), D, dtype=self.dtype, device=self.device)

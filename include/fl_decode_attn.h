@@ -235,7 +235,9 @@ int fl_prefill_mask_classify(const fl_attn_desc *desc, const float *attn_mask, i
  * is not full yet are kept in fp16 (rounded to nearest-even; non-finite values are stored as 0, finite ones kept
  * within +-65504) and quantised together when the block's last row arrives: scale = absmax / 127, integer =
  * rint(x * (127 / absmax)).  A row is therefore rounded to 8 bits once, and prompt pieces and decode steps may
- * fill a block in any mix.  The rows of a block share a scale: rows nobody attends to (padding) should be zeros,
+ * fill a block in any mix.  They append: a call's first row is the number of rows the cache holds, or one that starts
+ * again inside the open block or at a multiple of block_len (a row inside a complete block has its neighbours as bytes
+ * only; rows behind it go with it).  The rows of a block share a scale: rows nobody attends to (padding) should be zeros,
  * large ones cost their block-mates' precision.
  *
  * The calls take fl_attn_desc and fl_attn_io as the calls above do: desc.dtype is the type of q/k_new/v_new (int32
@@ -277,7 +279,8 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
                            int32_t weight_queries, void *hip_stream);
 
 /* The values of rows [0, rows) as [B,H,rows,D] in desc.dtype: to move a sequence to another cache type, to look at one.
- * rows_per_seq: NULL, or [B] on the device: rows from there on are zeros. */
+ * rows_per_seq: NULL where every sequence of the cache holds `rows` rows, or [B] on the device, how many each holds; rows
+ * from there on are zeros. */
 int fl_kv8_read(const fl_attn_desc *desc, const fl_kv8_cache *cache, int32_t rows, const int32_t *rows_per_seq,
                 void *k_out, void *v_out, void *hip_stream);
 
@@ -297,7 +300,7 @@ typedef struct fl_kv8_evict_args {
     int32_t to_total_len;        /* rows per (b,h) of `to`; 0 = desc.total_len */
     int32_t reserved;            /* 0 */
     int32_t *kept;               /* [B,H,keep_blocks]: the blocks that stay, ascending, -1 behind the last */
-    int32_t *rows_out;           /* [B]: rows after the eviction */
+    int32_t *rows_out;           /* [B]: rows after the eviction; not rows_per_seq */
 } fl_kv8_evict_args;
 int fl_kv8_evict(const fl_attn_desc *desc, const fl_kv8_cache *from, const fl_kv8_cache *to,
                  const fl_kv8_evict_args *args, void *hip_stream);

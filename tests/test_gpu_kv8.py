@@ -152,6 +152,21 @@ def test_a_row_that_sees_nothing_is_nan_and_gathers_nothing(gpu, D, rows):
         assert np.array_equal(after[:, :, :n], before[:, :, :n])
 
 
+@pytest.mark.parametrize("ready,nsplit", [(True, 1), (True, 3), (False, 3)])
+@pytest.mark.parametrize("rows", [0, 64, 384])
+def test_a_block_whose_first_row_sees_nothing_starts_from_zero(gpu, rows, ready, nsplit):
+    c = Case(gpu, 2, 2, 64, 512, 64, "f16", rows, weights=True, nsplit=nsplit)  # (behind the rows the weights are NaN)
+    if not ready:  # the merge as a launch of its own
+        def without(call, *args):
+            c.op.io.flags = 0
+            capi.check(call(*args, 0))
+        c.op._enqueue = without
+    got, want, tol = c.decode(np.full((512, 512), NEG, np.float32))
+    assert np.isnan(got.cpu().numpy()).all()
+    assert_cache(c.gpu, c.ref)
+    assert not c.gpu.weights[:, :, rows // 64].cpu().numpy().any()
+
+
 @pytest.mark.parametrize("ready", [True, False])
 @pytest.mark.parametrize("nsplit", [0, 2, 7, 1024])
 def test_decode_splits(gpu, nsplit, ready):
@@ -476,10 +491,11 @@ def test_read(gpu, D, T, dtype):
                 continue
             k, v = c.op.read(c.gpu, n, c.t(rows.astype(np.int32)) if ragged else None)
             for b in range(6):
-                for x, want in zip((k, v), c.ref.values(b, int(lens[b]))):
+                # (a row of a block that the sequence has completed is a byte row, wherever the output ends)
+                for x, want in zip((k, v), c.ref.values(b, int(rows[b]))):
                     x = x[b].cpu().numpy()
                     assert not x[:, lens[b]:].any()
-                    want = want.astype(np.float32).astype(x.dtype)
+                    want = want[:, :lens[b]].astype(np.float32).astype(x.dtype)
                     # (the fp16 value is that of the 32-bit product)
                     assert np.array_equal(x[:, :lens[b]], want)
 
@@ -507,6 +523,17 @@ def test_evict(gpu, D, T, keep, recent):
         g, want = (c.gpu, c.ref) if into is None else (to, into)
         for n in want.names():
             assert np.array_equal(bits(getattr(g, n).cpu().numpy()), bits(getattr(want, n))), (place, n)
+
+
+def test_read_of_fewer_rows_than_a_sequence_holds(gpu):
+    c = Case(gpu, 3, 2, 64, 192, 64, "f32", np.array([100, 191, 20]))
+    for n in (1, 40, 64, 70, 130):
+        k, v = c.op.read(c.gpu, n, c.t(c.rows.astype(np.int32)))
+        for b in range(3):
+            for x, want in zip((k, v), c.ref.values(b, int(c.rows[b]))):
+                m = min(n, int(c.rows[b]))
+                x = x[b].cpu().numpy()
+                assert np.array_equal(x[:, :m], want.astype(np.float32)[:, :m]) and not x[:, m:].any()
 
 
 def test_evict_many_blocks(gpu):

@@ -108,6 +108,8 @@ def test_decode_only_and_prompt_only():
     assert prefill(S=0) == capi.FL_ATTN_ERR_POSITION and prefill(S=254) == capi.FL_ATTN_ERR_POSITION
     assert prefill(W=-1) == capi.FL_ATTN_ERR_ARGUMENT
     assert prefill(d=desc(D=256)) == capi.FL_ATTN_ERR_HEAD_DIM  # weights beyond 128
+    wide = desc(B=64, H=64, D=256, L=8192)  # a workgroup per query: 2^32 threads
+    assert prefill(d=wide, c=fake_cache(weights=None), io=fake_io(start_pos=0), S=4096) == capi.FL_ATTN_ERR_SHAPE
     n = C.c_size_t()
     assert capi.load().fl_kv8_workspace_bytes(C.byref(desc()), 64, 257, C.byref(n)) == capi.FL_ATTN_ERR_POSITION
 
@@ -128,6 +130,8 @@ def test_read_refusals():
     (dict(kept=0x1002), capi.FL_ATTN_ERR_ALIGNMENT), (dict(rows_per_seq=0x1002), capi.FL_ATTN_ERR_ALIGNMENT),
     (dict(to_total_len=-64), capi.FL_ATTN_ERR_ARGUMENT), (dict(to_total_len=100), capi.FL_ATTN_ERR_SHAPE),
     (dict(to_total_len=128), capi.FL_ATTN_ERR_ARGUMENT),   # in place, another length
+    (dict(rows_per_seq=0x30004), capi.FL_ATTN_ERR_ARGUMENT), (dict(rows_per_seq=0x2003c), capi.FL_ATTN_ERR_ARGUMENT),  # written ranges
+    (dict(rows_out=0x2003c), capi.FL_ATTN_ERR_ARGUMENT),
     (dict(reserved=1), capi.FL_ATTN_ERR_ARGUMENT), (dict(struct_size=16), capi.FL_ATTN_ERR_STRUCT_SIZE),
 ])
 def test_evict_refusals(over, want):
