@@ -205,7 +205,7 @@ def load() -> C.CDLL:
     lib.fl_kv8_workspace_bytes.argtypes = [desc_p, C.c_int32, C.c_int32, size_p]
     lib.fl_kv8_workspace_init.argtypes = [desc_p, C.c_int32, C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]
     lib.fl_kv8_decode_forward.argtypes = [desc_p, cache_p, io_p, C.c_void_p, C.c_int32, C.c_void_p]
-    lib.fl_kv8_prefill_forward.argtypes = [desc_p, cache_p, io_p, C.c_int32, C.c_int32, C.c_void_p]
+    lib.fl_kv8_prefill_forward.argtypes = [desc_p, cache_p, io_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p]
     lib.fl_kv8_read.argtypes = [desc_p, cache_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
     lib.fl_kv8_evict.argtypes = [desc_p, cache_p, cache_p, C.POINTER(Kv8EvictArgs), C.c_void_p]
     lib.fl_kv8_cache_bytes.argtypes = [desc_p, C.c_int32, size_p, size_p, size_p]

@@ -372,8 +372,8 @@ int fl_kv8_decode_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, c
     return FL_ATTN_OK;
 }
 
-int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io_in, int32_t seq_len, int32_t weight_queries,
-                           void *hip_stream)
+int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io_in, int32_t seq_len, const int32_t *seq_len_per_seq,
+                           int32_t weight_queries, void *hip_stream)
 {
     fl_attn_desc desc_copy;
     int st = import_desc(&desc, &desc_copy);
@@ -386,7 +386,8 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
     if (st != FL_ATTN_OK) return st;
     st = check_io(&io);
     if (st != FL_ATTN_OK) return st;
-    if ((io.flags & ~FL_ATTN_IO_WORKSPACE_READY) != 0 || io.start_pos_per_seq || weight_queries < 0) return FL_ATTN_ERR_ARGUMENT; // uniform positions only
+    if ((io.flags & ~FL_ATTN_IO_WORKSPACE_READY) != 0 || io.start_pos_per_seq || weight_queries < 0) return FL_ATTN_ERR_ARGUMENT; // all start at one position
+    if ((reinterpret_cast<uintptr_t>(seq_len_per_seq) & 3u) != 0) return FL_ATTN_ERR_ALIGNMENT;
     const int L = desc->total_len, D = desc->size_per_head;
     if (seq_len < 1 || io.start_pos < 0 || (int64_t)io.start_pos + seq_len > L) return FL_ATTN_ERR_POSITION;
     if (io.attn_mask && (io.mask_ld < 0 || (io.mask_ld != 0 && io.mask_ld < (int64_t)io.start_pos + seq_len))) return FL_ATTN_ERR_ARGUMENT;
@@ -404,6 +405,7 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
     Kv8Params p = make_params(desc, &c, &io);
     p.a.out = io.out ? io.out : reinterpret_cast<float *>(ws + w.tmp_out);
     p.S = seq_len;
+    p.tokens_per_seq = seq_len_per_seq;
     Kv8PromptParams pp{};
     flattn::PrefillParams &f = pp.f;
     f.attn_mask = io.attn_mask; f.mask_ld = io.mask_ld;
@@ -419,8 +421,9 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
         p.weight_queries = weight_queries > 0 && weight_queries < seq_len ? weight_queries : seq_len;
         pp.q_pairs = reinterpret_cast<flattn::half8 *>(ws + w.q_pairs);
         pp.q_factor = reinterpret_cast<float *>(ws + w.q_factor);
-        pp.first_block = (seq_len - p.weight_queries) / 32;
-        pp.kept_blocks = (seq_len + 31) / 32 - pp.first_block;
+        // the last W queries lie in (W + 31) / 32 blocks where the sequence's end is a block's, else in one more
+        const int blocks = (seq_len + 31) / 32, spanned = seq_len_per_seq ? (p.weight_queries + 31) / 32 + 1 : blocks - (seq_len - p.weight_queries) / 32;
+        pp.kept_blocks = spanned < blocks ? spanned : blocks;
     }
     pp.key_splits = prompt_key_splits(desc, io.start_pos + seq_len, seq_len);
     if (pp.key_splits > 1) {

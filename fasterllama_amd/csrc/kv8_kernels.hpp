@@ -35,6 +35,7 @@ struct Kv8Params {
     int32_t T, t_shift;       // rows per block, log2
     int32_t nblk;             // L / T
     int32_t S;                // queries per sequence (prompt phase)
+    const int32_t *tokens_per_seq; // [B] how many of them are a sequence's own, or NULL: all
     float2 *stats;            // prompt phase, workspace [B*H, S]: (maximum, sum) of every query's softmax, or NULL
     int32_t weight_queries;   // the last of them whose weights are gathered
 };
@@ -280,6 +281,15 @@ __device__ __forceinline__ bool kv8_position_ok(const Kv8Params &p, int b, int P
     return !p.rope_rows || (uint32_t)p.rope_rows[b] < (uint32_t)p.table_rows;
 }
 
+// Tokens that sequence b brings to a prompt of S; -1 where its entry lies outside [0, S].
+__device__ __forceinline__ int kv8_prompt_tokens(const Kv8Params &p, int b)
+{
+    const int n = p.tokens_per_seq ? p.tokens_per_seq[b] : p.S;
+    return (uint32_t)n <= (uint32_t)p.S ? n : -1;
+}
+// What a query behind a sequence's tokens gets: zeros, or NaN where their number is unusable.
+__device__ __forceinline__ float kv8_no_query(int tokens) { return tokens < 0 ? __builtin_nanf("") : 0.f; }
+
 // Splits of one (b,h) in a decode step whose context is split: `chunk` rows of the complete blocks each, and one more for the
 // newest row and the open block's rows before it (or for the block that the newest row completes).
 __device__ __forceinline__ int kv8_splits(const Params &a, int T, int P) { return (P - (P & (T - 1)) + a.chunk - 1) / a.chunk + 1; }
@@ -326,7 +336,12 @@ void kv8_attn_kernel(const Kv8Params p)
         b = bs / p.S;
         s_query = bs % p.S;
         bh = b * H + h;
-        P = a.start_pos + p.S - 1; // the last row in the cache
+        const int tokens = kv8_prompt_tokens(p, b);
+        if (s_query >= tokens) {
+            for (int d = tid; d < D; d += kKv8Waves * 64) a.out[((size_t)bh * p.S + s_query) * D + d] = kv8_no_query(tokens);
+            return;
+        }
+        P = a.start_pos + tokens - 1; // the last row in the cache
     } else {
         const int BH = a.B * H;
         split = blockIdx.x / BH;
@@ -794,7 +809,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(const Kv8Params p)
     const int tid = threadIdx.x, bh = blockIdx.x % BH, b = bh / a.H, h = bh % a.H;
     const bool is_v = (blockIdx.x / BH & 1) != 0;
     const int nth = blockIdx.x / BH >> 1; // of the blocks this call touches
-    const int P = a.start_pos, end = P + p.S;
+    const int P = a.start_pos, end = P + max(kv8_prompt_tokens(p, b), 0);
     const int first = P / T, last = end / T;          // blocks [first, last) are complete after the call
     _Float16 *tail = (is_v ? p.v_tail : p.k_tail) + (size_t)bh * T * D;
     const void *src = is_v ? a.v_new : a.k_new;

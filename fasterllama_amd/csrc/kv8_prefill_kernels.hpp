@@ -34,8 +34,7 @@ struct Kv8PromptParams {
     PrefillParams f;      // mask, tile classes, B, H, L, S, start_pos
     half8 *q_pairs;       // workspace: rotated query operands of the last queries, for the block weights; or NULL
     float *q_factor;      // [B*H, query blocks of 32, 32] with them
-    int32_t first_block;  // 32-query blocks from here on are kept
-    int32_t kept_blocks;
+    int32_t kept_blocks;  // 32-query blocks of a sequence that they have room for; which ones: first_kept_block
     int32_t key_splits;   // workgroups that share the keys of a (query block, head); > 1: partials, merged by kv8_prompt_merge_kernel
     int32_t part_rows;    // queries per partial: 128, or the prompt's where it is shorter
     float *part_o;        // workspace [B*H * query blocks * splits, part_rows, D]: sums of weight * value, not normalised
@@ -63,6 +62,9 @@ __device__ __forceinline__ uint32_t prompt_class_word(const PrefillParams &f, in
         if (qb * kPrefillQueriesPerBlock + 32 * k < f.S) w |= kTileMixed << (8 * k);
     return w;
 }
+
+// The first 32-query block with one of the last weight_queries of a sequence's `tokens` queries.
+__device__ __forceinline__ int first_kept_block(const Kv8Params &p, int tokens) { return max(tokens - p.weight_queries, 0) / 32; }
 
 __device__ __forceinline__ void wave_lds_sync() // orders this wave's LDS writes and reads
 {
@@ -99,14 +101,23 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     int qb, bh;
     const int QB = (S + kPrefillQueriesPerBlock - 1) / kPrefillQueriesPerBlock, KS = pp.key_splits, split = (int)blockIdx.x / (QB * BH);
     prefill_block_to_tile((int)blockIdx.x % (QB * BH), BH, QB, HAS_MASK, qb, bh);
-    const int ctx = P + S, ctx8 = ctx & ~(p.T - 1); // rows [0, ctx8) are bytes, [ctx8, ctx) wait in the tail
-    const int NT = (ctx + BN - 1) / BN;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tokens = kv8_prompt_tokens(p, bh / a.H);
+    if (qb * kPrefillQueriesPerBlock >= tokens) { // none of the sequence's own (uniform)
+        if (KS > 1) return; // (the merge sees to them)
+        const int n = min(kPrefillQueriesPerBlock, S - qb * kPrefillQueriesPerBlock);
+        const float x = kv8_no_query(tokens);
+        float4 *dst = reinterpret_cast<float4 *>(a.out + ((size_t)bh * S + qb * kPrefillQueriesPerBlock) * D);
+        for (int i = tid; i < n * (D / 4); i += 256) dst[i] = make_float4(x, x, x, x);
+        return;
+    }
+    const int ctx = P + tokens, ctx8 = ctx & ~(p.T - 1); // rows [0, ctx8) are bytes, [ctx8, ctx) wait in the tail
+    const int NT = (ctx + BN - 1) / BN, class_ld = (P + S + BN - 1) / BN;
     const int qi = lane & 31, hf = lane >> 5;
     const int q_row = qb * kPrefillQueriesPerBlock + wave * 32 + qi;
 
     auto build_list = [&](int c0, int c1, bool have_first, uint32_t w_first) __attribute__((always_inline)) -> int {
-        return build_tile_list(pf, qb, c0, c1, NT, have_first, w_first, s_list, s_wave_cnt);
+        return build_tile_list(pf, qb, c0, c1, class_ld, have_first, w_first, s_list, s_wave_cnt);
     };
     // entry i of this workgroup's share, which starts at `share` of the pass's list
     int share = 0;
@@ -181,7 +192,7 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     if (split == 0) fetch(0); // a guess at the first listed tile: right without a mask and under every causal one
     uint32_t w_first = 0;
     if constexpr (HAS_MASK) {
-        if (tid < first_c1) w_first = prompt_class_word(pf, qb, tid, NT);
+        if (tid < first_c1) w_first = prompt_class_word(pf, qb, tid, class_ld);
     }
 
     // The rotated queries as fp16 pairs in operand layout, by way of LDS: every wave its own 32 (see the fp16 caches'
@@ -243,7 +254,7 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
 #pragma unroll
                         for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(__fmul_rn((float)(int)raw[jj][i / 4][i % 4], sc[jj]), ws[i]);
                     }
-                    const bool valid = q_first + q_rl(j0 + jj) < S;
+                    const bool valid = q_first + q_rl(j0 + jj) < tokens;
                     float *o = x[j0 + jj];
                     rope_pair(v[0], v[1], f[jj][0].x, f[jj][0].y, o[0], o[1]);
                     rope_pair(v[2], v[3], f[jj][0].z, f[jj][0].w, o[2], o[3]);
@@ -305,8 +316,8 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
         for (int c = 0; c < NC; ++c) qlo[c] = *reinterpret_cast<const half8 *>(sq + qi * LDQ + 16 * c + 8 * hf);
         const uint32_t e = qmax[qi] >> 23; // biased exponent of the largest element
         qc = a.scale * kLog2e * __uint_as_float((uint32_t)((int)e - 8) << 23);
-        const int block = q_first / 32 - pp.first_block;
-        if (pp.q_pairs && split == 0 && block >= 0 && q_first < S) { // kept for the block weights
+        const int block = q_first / 32 - first_kept_block(p, tokens);
+        if (pp.q_pairs && split == 0 && block >= 0 && q_first < tokens) { // kept for the block weights
             half8 *dst = pp.q_pairs + ((size_t)bh * pp.kept_blocks + block) * (2 * NC * 64) + lane;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -490,7 +501,7 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
 
     l += __shfl_xor(l, 32);
     const size_t slot = ((size_t)bh * QB + qb) * KS + split; // of the partials
-    if (hf == 0 && q_row < S) {
+    if (hf == 0 && q_row < tokens) {
         if (KS > 1) pp.part_ml[slot * pp.part_rows + wave * 32 + qi] = make_float2(m, l);
         else if (p.stats) p.stats[(size_t)bh * S + q_row] = make_float2(m, l);
     }
@@ -515,7 +526,8 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
 #pragma unroll
         for (int r0 = 0; r0 < 32; r0 += ROWS) {
             const int r = r0 + lane / LPRW, c4 = lane % LPRW;
-            const float4 v = *reinterpret_cast<const float4 *>(so + r * LDO + 4 * c4);
+            float4 v = *reinterpret_cast<const float4 *>(so + r * LDO + 4 * c4);
+            if (q0 + r >= tokens) v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (q0 + r < S) *reinterpret_cast<float4 *>(dst0 + (size_t)r * D + pass * HALF_D + 4 * c4) = v;
         }
         wave_lds_sync(); // the slice is rewritten by the next pass
@@ -533,6 +545,12 @@ __global__ __launch_bounds__(256) void kv8_prompt_merge_kernel(const Kv8PromptPa
     const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
     if (threadIdx.x >= ROWS * TPR || row >= (int64_t)p.a.B * p.a.H * S) return;
     const int bh = (int)(row / S), q = (int)(row % S), t = threadIdx.x % TPR;
+    const int tokens = kv8_prompt_tokens(p, bh / p.a.H);
+    if (q >= tokens) {
+        const float x = kv8_no_query(tokens);
+        reinterpret_cast<float4 *>(p.a.out + (size_t)row * D)[t] = make_float4(x, x, x, x);
+        return;
+    }
     const size_t slot0 = ((size_t)bh * QB + q / kPrefillQueriesPerBlock) * KS, at = q % kPrefillQueriesPerBlock;
     float M = kMaxFloor * kLog2e;
     for (int s = 0; s < KS; ++s) M = fmaxf(M, pp.part_ml[(slot0 + s) * pp.part_rows + at].x);
@@ -557,7 +575,7 @@ __global__ __launch_bounds__(256) void kv8_prompt_merge_kernel(const Kv8PromptPa
 // query and key; what bounds it is reading the queries' operands, 16 KB per 32 of them at D = 128.  A wave keeps 64 keys in
 // registers, and the four waves of a workgroup are 4 / NQ groups of keys times NQ streams of queries: with NQ = 1 they read
 // the same operands together, with NQ = 4 a workgroup is done sooner, where there are few of them.  grid = ceil(keys / (256 / NQ))
-// * B*H, block = 256.  Sums are formed in one order, so they are the same from run to run.
+// * B*H of the longest sequence, block = 256.  Sums are formed in one order, so they are the same from run to run.
 template <int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 8)))
 void kv8_prompt_weights_kernel(const Kv8PromptParams pp, int NQ)
@@ -566,9 +584,11 @@ void kv8_prompt_weights_kernel(const Kv8PromptParams pp, int NQ)
     __shared__ float s_sum[4][KT];
     const Kv8Params &p = pp.k;
     const Params &a = p.a;
-    const int S = p.S, P = a.start_pos, T = p.T, ctx = P + S, ctx8 = ctx & ~(T - 1), NT = (ctx + 31) / 32;
-    const int keys = 256 / NQ, groups = (ctx + keys - 1) / keys;
+    const int S = p.S, P = a.start_pos, T = p.T, class_ld = (P + S + 31) / 32;
+    const int keys = 256 / NQ, groups = (P + S + keys - 1) / keys;
     const int wg_key = blockIdx.x % groups * keys, bh = blockIdx.x / groups;
+    const int tokens = kv8_prompt_tokens(p, bh / a.H), ctx = P + tokens, ctx8 = ctx & ~(T - 1);
+    if (tokens <= 0 || wg_key >= ctx) return; // (uniform)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qi = lane & 31, hf = lane >> 5;
     const int key0 = wg_key + wave / NQ * (32 * KT); // this wave's first key
     half8 ka[KT][NC]; // key key0 + 32 t + qi, elements 16c + 8hf ..
@@ -599,16 +619,16 @@ void kv8_prompt_weights_kernel(const Kv8PromptParams pp, int NQ)
             }
         }
     }
-    const int first_query = S - p.weight_queries;
+    const int first_query = tokens - p.weight_queries, first_block = first_kept_block(p, tokens), blocks = (tokens + 31) / 32 - first_block;
     float sum[KT] = {0.f, 0.f};
-    for (int block = key0 < ctx ? wave % NQ : pp.kept_blocks; block < pp.kept_blocks; block += NQ) {
-        const int q0 = (pp.first_block + block) * 32;
+    for (int block = key0 < ctx ? wave % NQ : blocks; block < blocks; block += NQ) {
+        const int q0 = (first_block + block) * 32;
         uint32_t cls[KT];
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             cls[t] = kTileSkip;
             if (key0 + 32 * t < ctx)
-                cls[t] = a.attn_mask ? (prompt_class_word(pp.f, q0 / kPrefillQueriesPerBlock, key0 / 32 + t, NT) >> (8 * (q0 / 32 % 4))) & 0xffu : kTileZero;
+                cls[t] = a.attn_mask ? (prompt_class_word(pp.f, q0 / kPrefillQueriesPerBlock, key0 / 32 + t, class_ld) >> (8 * (q0 / 32 % 4))) & 0xffu : kTileZero;
             cls[t] = __builtin_amdgcn_readfirstlane(cls[t]);
         }
         if (cls[0] == kTileSkip && cls[1] == kTileSkip) continue;
@@ -624,7 +644,7 @@ void kv8_prompt_weights_kernel(const Kv8PromptParams pp, int NQ)
         const float2 ml = p.stats[(size_t)bh * S + q_in];
         const float factor = pp.q_factor[kept * 32 + qi];
         // a query of the call that counts, and that saw a key
-        const float rl = q >= first_query && q < S && ml.y > 0.f ? 1.0f / ml.y : 0.f;
+        const float rl = q >= first_query && q < tokens && ml.y > 0.f ? 1.0f / ml.y : 0.f;
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             if (cls[t] == kTileSkip) continue;

@@ -185,9 +185,10 @@ class KV8Attention:
 
     def prefill(self, q, k_new, v_new, cache: KV8Cache, freq_cis, start_pos: int = 0, attn_mask=None, mask_tile_classes=None,
                 rope_row: int = capi.FL_ATTN_ROPE_AT_POSITION, weight_queries: int = 0, scales=None, out=None, out_int8=None,
-                out_scale=None):
+                out_scale=None, seq_len_per_seq=None):
         """The prompt phase: q, k_new, v_new [B,S,H,D] at positions start_pos .. start_pos+S-1 (causal by the mask); returns
-        out [B,H,S,D] float32.  With cache.weights, the last weight_queries queries add theirs (0: all).  mask_tile_classes:
+        out [B,H,S,D] float32.  seq_len_per_seq: int32 [B] on the device, the tokens that each sequence brings of them: the
+        padding behind is not stored, its output rows are zeros.  With cache.weights, the last weight_queries queries add theirs (0: all).  mask_tile_classes:
         PrefillAttention.classify_mask of the whole [L, L] mask."""
         B, H, L, D = self.shape
         S = q.shape[1] if q.dim() == 4 else 0
@@ -203,7 +204,8 @@ class KV8Attention:
         else:
             n = -(-L // 32)
             io.mask_tile_classes = self._vector("mask_tile_classes", mask_tile_classes, torch.uint8, n * -(-n // 4) * 4)
-        self._enqueue(self.lib.fl_kv8_prefill_forward, self._desc, cache.ref, self._io, S, weight_queries)
+        self._enqueue(self.lib.fl_kv8_prefill_forward, self._desc, cache.ref, self._io, S,
+                      self._vector("seq_len_per_seq", seq_len_per_seq, torch.int32, B), weight_queries)
         return out
 
     def read(self, cache: KV8Cache, rows: int, rows_per_seq=None):

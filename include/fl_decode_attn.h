@@ -273,10 +273,14 @@ int fl_kv8_workspace_init(const fl_attn_desc *desc, int32_t block_len, int32_t s
 int fl_kv8_decode_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io,
                           const int32_t *rope_row_per_seq, int32_t rope_table_rows, void *hip_stream);
 
-/* The prompt phase (layouts and mask as fl_prefill_attn_forward).  With cache.weights, the last weight_queries queries
- * of every sequence add theirs (0 = all); served for size_per_head <= 128 (FL_ATTN_ERR_HEAD_DIM). */
+/* The prompt phase (layouts and mask as fl_prefill_attn_forward).  seq_len_per_seq: NULL, or [B] on the device: sequence b
+ * brings its first seq_len_per_seq[b] <= seq_len tokens (0: none).  What pads it behind them is not stored and nobody
+ * attends to it, and its output rows are zeros; the next row of that sequence is start_pos + seq_len_per_seq[b].  An entry
+ * outside [0, seq_len]: NaN output for that sequence, nothing stored.  (A padded prompt without it is stored whole, and its
+ * padding cannot be overwritten row by row: see the order of appends above.)  With cache.weights, the last weight_queries
+ * queries of every sequence add theirs (0 = all); served for size_per_head <= 128 (FL_ATTN_ERR_HEAD_DIM). */
 int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io, int32_t seq_len,
-                           int32_t weight_queries, void *hip_stream);
+                           const int32_t *seq_len_per_seq, int32_t weight_queries, void *hip_stream);
 
 /* The values of rows [0, rows) as [B,H,rows,D] in desc.dtype: to move a sequence to another cache type, to look at one.
  * rows_per_seq: NULL where every sequence of the cache holds `rows` rows, or [B] on the device, how many each holds; rows

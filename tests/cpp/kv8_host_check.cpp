@@ -53,15 +53,15 @@ int main()
                             io.freq_cis = (const float *)at(0x1000); io.out = (float *)at(0x1000);
                             io.start_pos = d.total_len; io.rope_row = -1; io.max_start_pos = -1;
                             EXPECT(fl_kv8_decode_forward(&d, &c, &io, nullptr, 0, nullptr) == FL_ATTN_ERR_POSITION);
-                            EXPECT(fl_kv8_prefill_forward(&d, &c, &io, 1, 0, nullptr) == FL_ATTN_ERR_POSITION);
+                            EXPECT(fl_kv8_prefill_forward(&d, &c, &io, 1, nullptr, 0, nullptr) == FL_ATTN_ERR_POSITION);
                             io.start_pos = 0; // no workspace
                             EXPECT(fl_kv8_decode_forward(&d, &c, &io, nullptr, 0, nullptr) == FL_ATTN_ERR_WORKSPACE);
-                            EXPECT(fl_kv8_prefill_forward(&d, &c, &io, 1, 0, nullptr) == (D > 128 ? FL_ATTN_ERR_HEAD_DIM : FL_ATTN_ERR_WORKSPACE));
+                            EXPECT(fl_kv8_prefill_forward(&d, &c, &io, 1, nullptr, 0, nullptr) == (D > 128 ? FL_ATTN_ERR_HEAD_DIM : FL_ATTN_ERR_WORKSPACE));
                             EXPECT(fl_kv8_read(&d, &c, 0, nullptr, at(0x1000), at(0x2000), nullptr) == FL_ATTN_ERR_POSITION);
                             fl_kv8_evict_args e;
                             std::memset(&e, 0, sizeof e);
                             e.struct_size = sizeof e;
-                            e.keep_blocks = blocks + 1; e.kept = (int32_t *)at(0x1000); e.rows_out = (int32_t *)at(0x1000);
+                            e.keep_blocks = blocks + 1; e.kept = (int32_t *)at(0x80000000000); e.rows_out = (int32_t *)at(0x1000);
                             EXPECT(fl_kv8_evict(&d, &c, &c, &e, nullptr) == FL_ATTN_ERR_ARGUMENT);
                             e.keep_blocks = 1;
                             fl_kv8_cache to = c;

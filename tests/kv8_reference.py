@@ -87,30 +87,33 @@ class Cache:
             out.append(x)
         return out
 
-    def step(self, q, k_new, v_new, table, start, mask=None, rope=None, scale=None, weight_queries=0):
-        """S tokens [B,S,H,D] at rows start[b] ..; returns out [B,H,S,D] and how far a 32-bit computation may be off it
+    def step(self, q, k_new, v_new, table, start, mask=None, rope=None, scale=None, weight_queries=0, lens=None):
+        """S tokens [B,S,H,D] at rows start[b] .., lens[b] of them the sequence's own; returns out [B,H,S,D] and how far a 32-bit computation may be off it
         [B,1,1,1] (see tolerance()).  A position outside the cache: NaN, nothing stored."""
-        B, S, H, D = q.shape
+        B, S_all, H, D = q.shape
         scale = scale or 1.0 / math.sqrt(D)
-        out, tol = np.full((B, H, S, D), np.nan), np.zeros((B, 1, 1, 1))
+        out, tol = np.full((B, H, S_all, D), np.nan), np.zeros((B, 1, 1, 1))
         for b in range(B):
-            P = int(start[b])
-            if P < 0 or P + S > self.L:
+            P, S = int(start[b]), S_all if lens is None else int(lens[b])
+            if P < 0 or P + S > self.L or S < 0 or S > S_all:
+                continue
+            out[b] = 0.0
+            if S == 0:
                 continue
             rr = P if rope is None else int(rope[b])
             rows = table[rr:rr + S][:, None]
-            kk, vv = stored(rotate_key(k_new[b], rows)), stored(v_new[b])
+            kk, vv = stored(rotate_key(k_new[b, :S], rows)), stored(v_new[b, :S])
             for s in range(S):
                 self.put(b, P + s, kk[s], vv[s])
             k, v = self.values(b, P + S)
-            qq = rotate(q[b], rows).transpose(1, 0, 2)
+            qq = rotate(q[b, :S], rows).transpose(1, 0, 2)
             z = qq @ k.transpose(0, 2, 1) * scale
             with np.errstate(invalid="ignore", over="ignore"):
                 if mask is not None:
                     z = z + mask[P:P + S, :P + S].astype(np.float64)
                 e = np.exp(z - np.maximum(z.max(-1, keepdims=True), -1e9))
                 p = e / e.sum(-1, keepdims=True)
-                out[b] = p @ v
+                out[b, :, :S] = p @ v
             tol[b] = self.tolerance(qq, k, v, scale, P + S)
             if self.weights is not None:
                 W = min(weight_queries or S, S)

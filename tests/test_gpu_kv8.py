@@ -331,6 +331,43 @@ def test_prompt_masks(gpu, kind, start, S):
     assert_cache(c.gpu, c.ref, S, start + S)
 
 
+@pytest.mark.parametrize("D,T,dtype", [(128, 64, "f16"), (96, 32, "f32"), (32, 128, "i32"), (256, 64, "f16")])
+@pytest.mark.parametrize("kind", [None, "causal"])
+@pytest.mark.parametrize("start,S", [(0, 300), (77, 130), (13, 60), (1100, 40)])
+def test_padded_prompts_of_different_lengths(gpu, D, T, dtype, kind, start, S):
+    """The padding (NaN here) is neither stored nor read; rows behind a sequence's own are left as they were."""
+    import torch
+    lens = np.array([S, 0, 1, S // 2, S + 1, -1, 32, S - 1], np.int32)
+    L = 1152 if start > 1000 else 384
+    c = Case(gpu, 8, 2, D, L, T, dtype, start, weights=D <= 128, max_seq_len=S)
+    raw, val, sc = c.feed(S, 11)
+    for b in range(8):
+        for x in raw:
+            x[b, max(lens[b], 0):] = 2 ** 30 if dtype == "i32" else float("nan")
+    m = masks(kind, L)
+    before = {n: getattr(c.gpu, n).cpu().numpy().copy() for n in c.ref.names()}
+    got = c.op.prefill(*raw, c.gpu, c.table_d, start_pos=start, attn_mask=c.t(m), scales=sc, weight_queries=20, seq_len_per_seq=c.t(lens))
+    want, tol = c.ref.step(*val, c.table, c.rows, m, weight_queries=20, lens=lens)
+    assert_out(got, want, tol, f"D {D} start {start} S {S}")
+    for b in range(8):
+        assert not got[b, :, max(lens[b], 0):].cpu().numpy().any() or lens[b] not in range(S + 1)
+    n = np.where((lens < 0) | (lens > S), 0, lens) + start
+    for b in range(8):
+        for name in c.ref.names():
+            x, ref = getattr(c.gpu, name)[b].cpu().numpy(), getattr(c.ref, name)[b]
+            if name == "weights":
+                ok = ~np.isnan(ref)
+                assert np.array_equal(np.isnan(x), ~ok) and (np.abs(x[ok] - ref[ok]) <= 2e-5 * 20 * np.maximum(1.0, np.abs(ref[ok]))).all(), b
+            elif name.endswith("_tail"):
+                assert np.array_equal(bits(x[:, :n[b] % T]), bits(ref[:, :n[b] % T])), (b, name)
+            else:
+                assert np.array_equal(bits(x), bits(ref)), (b, name)
+    # and every sequence decodes on from its own length
+    c.rows = np.where((lens < 0) | (lens > S), -1, n)
+    got, want, tol = c.decode(ragged=True, seed=12, bound=start + S)
+    assert_out(got, want, tol, "step")
+
+
 @pytest.mark.parametrize("dtype", ["f16", "i32"])
 def test_prompt_in_pieces_and_steps_leaves_the_same_bits(gpu, dtype):
     """Rows, scales and tails do not depend on how the rows arrived."""

@@ -38,8 +38,8 @@ def decode(d=None, c=None, io=None, rope=None, rows=64):
     return capi.load().fl_kv8_decode_forward(C.byref(d or desc()), C.byref(c or fake_cache()), C.byref(io or fake_io()), rope, rows, None)
 
 
-def prefill(d=None, c=None, io=None, S=8, W=0):
-    return capi.load().fl_kv8_prefill_forward(C.byref(d or desc()), C.byref(c or fake_cache()), C.byref(io or fake_io()), S, W, None)
+def prefill(d=None, c=None, io=None, S=8, W=0, lens=None):
+    return capi.load().fl_kv8_prefill_forward(C.byref(d or desc()), C.byref(c or fake_cache()), C.byref(io or fake_io()), S, lens, W, None)
 
 
 def evict(d=None, c=None, to=None, **over):
@@ -107,6 +107,7 @@ def test_decode_only_and_prompt_only():
     assert prefill(io=fake_io(start_pos_per_seq=0x1000)) == capi.FL_ATTN_ERR_ARGUMENT
     assert prefill(S=0) == capi.FL_ATTN_ERR_POSITION and prefill(S=254) == capi.FL_ATTN_ERR_POSITION
     assert prefill(W=-1) == capi.FL_ATTN_ERR_ARGUMENT
+    assert prefill(lens=0x1002) == capi.FL_ATTN_ERR_ALIGNMENT
     assert prefill(d=desc(D=256)) == capi.FL_ATTN_ERR_HEAD_DIM  # weights beyond 128
     wide = desc(B=64, H=64, D=256, L=8192)  # a workgroup per query: 2^32 threads
     assert prefill(d=wide, c=fake_cache(weights=None), io=fake_io(start_pos=0), S=4096) == capi.FL_ATTN_ERR_SHAPE
