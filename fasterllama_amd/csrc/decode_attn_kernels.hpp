@@ -250,9 +250,9 @@ __device__ __forceinline__ void store_partial(float *p, float v)
 //   M = max_s m_s;  w_s = exp(m_s - M);  out[d] = sum_s w_s o_s[d] / sum_s w_s l_s.
 // The weights are computed once per split (threads over s), then the weighted sum over splits runs
 // with D/4 threads per split-group (float4 per thread) and 256/(D/4) split-groups side by side, so
-// the partial loads of a group are independent and in flight together.  Returns (M, sum_s w_s l_s), in every thread.
+// the partial loads of a group are independent and in flight together.
 template <int D, bool DEVICE_COHERENT>
-__device__ __forceinline__ float2 combine_partials(const Params &p, int bh, int nsp, int tid, CombineShared<D> &sh)
+__device__ __forceinline__ void combine_partials(const Params &p, int bh, int nsp, int tid, CombineShared<D> &sh)
 {
     constexpr int TPG = CombineShared<D>::TPG, SG = CombineShared<D>::SG;
     constexpr int VPT = D / 4 / TPG; // float4 per thread
@@ -352,7 +352,6 @@ __device__ __forceinline__ float2 combine_partials(const Params &p, int bh, int 
         r.x = r.x / Lsum; r.y = r.y / Lsum; r.z = r.z / Lsum; r.w = r.w / Lsum;
         reinterpret_cast<float4 *>(p.out + (size_t)bh * D)[d4] = r;
     }
-    return make_float2(M, Lsum);
 }
 
 // Splits of one (b,h) that stream rows (the others return at once): ceil((P+1)/chunk), which is at most

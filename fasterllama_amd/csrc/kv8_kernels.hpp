@@ -40,6 +40,10 @@ struct Kv8Params {
     int32_t weight_queries;   // the last of them whose weights are gathered
 };
 
+// A uniform value of an input that no kernel writes while this one runs, by a scalar load.
+template <typename T>
+__device__ __forceinline__ T load_uniform(const T *p) { return *(const __attribute__((address_space(4))) T *)p; }
+
 // ---------------------------------------------------------------- inputs and stored values
 
 // N consecutive elements of an input tensor as float.  The input format is uniform: one straight run of loads each.
@@ -192,6 +196,31 @@ __device__ __forceinline__ float cross_sum(float x)
     return x;
 }
 
+// Sums 16 values per lane over the lane groups and leaves a lane with a share of the sums, x[0 .. result) of elements
+// 8 * (lane / 32) + 4 * (lane / 16 % 2) + i (rows of more lanes: the larger share): the first two steps exchange what the other half
+// keeps, one instruction for two values, and the last ones have a quarter of the values to add.
+template <int LPR>
+__device__ __forceinline__ constexpr int scattered() { return LPR <= 16 ? 4 : (LPR <= 32 ? 8 : 16); }
+template <int LPR>
+__device__ __forceinline__ void scatter_sum(float (&x)[16])
+{
+    auto add = [](auto r) __attribute__((always_inline)) -> float { return __uint_as_float(r[0]) + __uint_as_float(r[1]); };
+    if constexpr (LPR <= 32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = add(__builtin_amdgcn_permlane32_swap(__float_as_uint(x[i]), __float_as_uint(x[i + 8]), false, false));
+    }
+    if constexpr (LPR <= 16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = add(__builtin_amdgcn_permlane16_swap(__float_as_uint(x[i]), __float_as_uint(x[i + 4]), false, false));
+    }
+#pragma unroll
+    for (int i = 0; i < scattered<LPR>(); ++i) {
+        if constexpr (LPR <= 8) x[i] += dpp_move<0x128>(x[i]); // lane ^ 8
+        if constexpr (LPR <= 4) x[i] += __shfl_xor(x[i], 4);
+        if constexpr (LPR <= 2) x[i] += dpp_move<0x4E>(x[i]);  // lane ^ 2
+    }
+}
+
 // ---------------------------------------------------------------- decode step
 
 template <int D>
@@ -211,10 +240,29 @@ constexpr float kKv8LazyMax = 8.0f; // base-2 units: the running reference maxim
 constexpr float kQDigits = 8300000.0f; // |q| maps to at most this: three balanced base-256 digits reach 8355711
 constexpr int kKv8Waves = 4;
 
+// What thread tid needs of its first block (block tid) for the block weights: the weight so far and, where a block is at most
+// four granules, those.  Requested ahead of the merge, whose loads they travel with.
+template <int D>
+struct FirstBlock {
+    static constexpr int GR = Kv8Geometry<D>::GR, N = GR == 32 ? 4 : 0;
+    float old;
+    float2 g[N ? N : 1];
+    template <typename LOAD>
+    __device__ __forceinline__ void request(const Kv8Params &p, int bh, int P, int tid, LOAD granule)
+    {
+        old = 0.f;
+        if (tid > P >> p.t_shift) return;
+        old = p.weights[(size_t)bh * p.nblk + tid];
+        const int per = p.T / GR;
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] = granule(tid * per + min(i, per - 1)); // (those that nobody wrote are not used)
+    }
+};
+
 // Adds the softmax weight of every block to weights[b,h,:], from the granules and the merged statistics (M, Lsum) of the
-// row.  A block whose first row arrived in this step starts from 0.  old: this thread's first block's weight so far.
-template <int D, typename LOAD>
-__device__ __forceinline__ void add_block_weights(const Kv8Params &p, int bh, int P, float M, float Lsum, int tid, LOAD granule, float old)
+// row.  A block whose first row arrived in this step starts from 0.
+template <int D, bool AHEAD, typename LOAD>
+__device__ __forceinline__ void add_block_weights(const Kv8Params &p, int bh, int P, float M, float Lsum, int tid, LOAD granule, const FirstBlock<D> &first)
 {
     constexpr int GR = Kv8Geometry<D>::GR;
     const int blk_new = P >> p.t_shift;
@@ -228,13 +276,19 @@ __device__ __forceinline__ void add_block_weights(const Kv8Params &p, int bh, in
     for (int blk = tid; blk <= blk_new; blk += kKv8Waves * 64) {
         float w = 0.f;
         const int n = open && blk == blk_new ? 1 : per;
-        for (int i = 0; i < n; ++i) {
-            const float2 ms = granule(blk * per + i);
-            w = fmaf(ms.y, __builtin_amdgcn_exp2f(ms.x - M), w);
+        if (AHEAD && FirstBlock<D>::N > 0 && blk == tid) {
+#pragma unroll
+            for (int i = 0; i < FirstBlock<D>::N; ++i)
+                if (i < n) w = fmaf(first.g[i].y, __builtin_amdgcn_exp2f(first.g[i].x - M), w);
+        } else {
+            for (int i = 0; i < n; ++i) {
+                const float2 ms = granule(blk * per + i);
+                w = fmaf(ms.y, __builtin_amdgcn_exp2f(ms.x - M), w);
+            }
         }
         float *dst = p.weights + (size_t)bh * p.nblk + blk;
         const bool fresh = blk == blk_new && (P & (p.T - 1)) == 0;
-        *dst = fresh ? w * rl : fmaf(w, rl, blk == tid ? old : *dst);
+        *dst = fresh ? w * rl : fmaf(w, rl, blk == tid ? first.old : *dst);
     }
 }
 
@@ -244,6 +298,75 @@ struct GranuleLoader {
     __device__ __forceinline__ float2 operator()(int i) const { return make_float2(load_partial<true>(at + 2 * i), load_partial<true>(at + 2 * i + 1)); }
 };
 __device__ __forceinline__ GranuleLoader granule_loader(const float2 *at) { return GranuleLoader{reinterpret_cast<const float *>(at)}; }
+
+// Merges the (m, l, o[D]) partials of the nsp splits of one (b,h), by the 256 threads of a workgroup, into a.out:
+//   M = max_s m_s;  w_s = 2^(m_s - M);  out[d] = sum_s w_s o_s[d] / sum_s w_s l_s.
+// D/4 threads take a split's row, 256 / (D/4) rows side by side.  Every wave forms the weights for itself, lane s that of split s,
+// so that nothing but the last sum crosses waves: one memory round trip and one barrier.  COHERENT: loads that go past the
+// caches which are private to a compute unit or an XCD, 16 bytes each (8 heads, 4000 rows, 33 splits: 9.3 us the step, with
+// single words 9.9; with the three barriers of the other caches' merge and the weights' loads behind it 11.1; 32 heads, 1000 rows:
+// 8.9 against 10.1).  Returns (M, sum of w_s l_s), in every thread.
+constexpr int kLoadDeviceCoherent = 16; // cache-policy bits of the buffer builtins: bit 4 = sc1, as a device-scope atomic load has it
+template <int D>
+struct MergeShared {
+    static constexpr int TPG = D / 4, SG = 256 / TPG; // threads per split, splits side by side (size_per_head 96: 16 threads left over)
+    static constexpr int PRE = 64 / SG < 4 ? 64 / SG : 4; // rows requested with the statistics; their weights lie in one wave's lanes
+    float4 acc[SG][TPG];
+    float w[kCombineMaxSplits];
+};
+template <int D, bool COHERENT>
+__device__ __forceinline__ float2 kv8_merge(const Params &a, int bh, int nsp, int tid, MergeShared<D> &sh)
+{
+    constexpr int TPG = MergeShared<D>::TPG, SG = MergeShared<D>::SG, PRE = MergeShared<D>::PRE, POLICY = COHERENT ? kLoadDeviceCoherent : 0;
+    const int lane = tid & 63, sg = tid / TPG, t = tid % TPG;
+    const bool in_group = SG * TPG == kCombineThreads || sg < SG;
+    const size_t slot0 = (size_t)bh * a.split_cap;
+    const __amdgpu_buffer_rsrc_t Obuf = make_buffer(a.part_o + slot0 * D), Mbuf = make_buffer(a.part_m + slot0), Lbuf = make_buffer(a.part_l + slot0);
+    auto stat = [&](__amdgpu_buffer_rsrc_t buf, int s) __attribute__((always_inline)) -> float { // 0 behind the last
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buf, s < nsp ? (uint32_t)s * 4u : kLaneOutOfRange, 0u, POLICY));
+    };
+    auto row = [&](int s) __attribute__((always_inline)) -> float4 {
+        return __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(Obuf, in_group && s < nsp ? (uint32_t)(s * TPG + t) * 16u : kLaneOutOfRange, 0u, POLICY));
+    };
+    const float m0 = stat(Mbuf, lane), l0 = stat(Lbuf, lane);
+    float4 x[PRE];
+#pragma unroll
+    for (int k = 0; k < PRE; ++k) x[k] = row(sg + k * SG);
+    __builtin_amdgcn_sched_barrier(0);
+
+    float M = lane < nsp ? m0 : kMaxFloor * kLog2e;
+    for (int s = lane + 64; s < nsp; s += 64) M = fmaxf(M, stat(Mbuf, s));
+    M = wave_max(M);
+    const float w = lane < nsp ? __builtin_amdgcn_exp2f(m0 - M) : 0.f;
+    float Lsum = l0 * w;
+    for (int s = lane + 64; s < nsp; s += 64) Lsum = fmaf(stat(Lbuf, s), __builtin_amdgcn_exp2f(stat(Mbuf, s) - M), Lsum);
+    Lsum = wave_sum(Lsum);
+
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float4 y, float ws) __attribute__((always_inline)) {
+        acc.x = fmaf(y.x, ws, acc.x); acc.y = fmaf(y.y, ws, acc.y); acc.z = fmaf(y.z, ws, acc.z); acc.w = fmaf(y.w, ws, acc.w);
+    };
+#pragma unroll
+    for (int k = 0; k < PRE; ++k) add(x[k], __shfl(w, (sg + k * SG) & 63)); // (zeros behind the last)
+    if (nsp > PRE * SG) { // uniform
+        for (int s = tid; s < nsp; s += kCombineThreads) sh.w[s] = __builtin_amdgcn_exp2f(stat(Mbuf, s) - M);
+        __syncthreads();
+#pragma unroll 4
+        for (int s = sg + PRE * SG; s < nsp; s += SG) add(row(s), sh.w[s]);
+    }
+    if (in_group) sh.acc[sg][t] = acc;
+    __syncthreads();
+    if (tid < TPG) {
+        float4 r = sh.acc[0][tid];
+#pragma unroll
+        for (int k = 1; k < SG; ++k) {
+            const float4 y = sh.acc[k][tid];
+            r.x += y.x; r.y += y.y; r.z += y.z; r.w += y.w;
+        }
+        reinterpret_cast<float4 *>(a.out + (size_t)bh * D)[tid] = make_float4(r.x / Lsum, r.y / Lsum, r.z / Lsum, r.w / Lsum);
+    }
+    return make_float2(M, Lsum);
+}
 
 // Quantises one full tail (T rows of one (b,h)) into block `blk`, by the 256 threads of a workgroup.  Two passes over
 // the tail: T * D halfs, which the second finds in the caches.
@@ -278,13 +401,13 @@ __device__ __forceinline__ void quantise_tail(const _Float16 *tail, int8_t *rows
 __device__ __forceinline__ bool kv8_position_ok(const Kv8Params &p, int b, int P)
 {
     if (P < 0 || P >= p.a.L || P > p.a.max_pos) return false;
-    return !p.rope_rows || (uint32_t)p.rope_rows[b] < (uint32_t)p.table_rows;
+    return !p.rope_rows || (uint32_t)load_uniform(p.rope_rows + b) < (uint32_t)p.table_rows;
 }
 
 // Tokens that sequence b brings to a prompt of S; -1 where its entry lies outside [0, S].
 __device__ __forceinline__ int kv8_prompt_tokens(const Kv8Params &p, int b)
 {
-    const int n = p.tokens_per_seq ? p.tokens_per_seq[b] : p.S;
+    const int n = p.tokens_per_seq ? load_uniform(p.tokens_per_seq + b) : p.S;
     return (uint32_t)n <= (uint32_t)p.S ? n : -1;
 }
 // What a query behind a sequence's tokens gets: zeros, or NaN where their number is unusable.
@@ -321,11 +444,14 @@ void kv8_attn_kernel(const Kv8Params p)
     static_assert(kKv8Waves * 64 == kCombineThreads, "the merge runs on a 256-thread workgroup");
     __shared__ float s_o[kKv8Waves][D];
     __shared__ float s_m[kKv8Waves], s_l[kKv8Waves], s_t[kKv8Waves], s_red[kKv8Waves];
-    __shared__ __attribute__((aligned(16))) char s_merge_bytes[PROMPT ? 16 : sizeof(CombineShared<D>)];
+    __shared__ __attribute__((aligned(16))) char s_merge_bytes[PROMPT ? 16 : sizeof(MergeShared<D>)];
     constexpr int LDS_GRANULES = (int)sizeof(s_merge_bytes) / 8; // where one workgroup has all rows and does not merge
     __shared__ int s_last;
 
     const Params &a = p.a;
+    // One argument of every 64-byte line at once: fetched where they are first used, the lines cost three more scalar round trips
+    // before the first request (0.1-0.2 us).
+    asm volatile("" ::"s"(a.q), "s"(p.k8), "s"(p.in_kind), "s"(p.T));
     const int H = a.H, L = a.L, T = p.T;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane / LPR, lig = lane % LPR;
@@ -348,7 +474,7 @@ void kv8_attn_kernel(const Kv8Params p)
         bh = blockIdx.x % BH;
         b = bh / H;
         h = bh % H;
-        P = a.pos_per_seq ? a.pos_per_seq[b] : a.start_pos;
+        P = a.pos_per_seq ? load_uniform(a.pos_per_seq + b) : a.start_pos;
         if (!kv8_position_ok(p, b, P)) { // store nothing, poison the output
             if ((a.direct || a.arrivals) && split == 0)
                 for (int d = tid; d < D; d += kKv8Waves * 64) a.out[(size_t)bh * D + d] = __builtin_nanf("");
@@ -369,9 +495,9 @@ void kv8_attn_kernel(const Kv8Params p)
     const int e0 = lig * 16, e0_in = has_chunk ? e0 : 0; // (lanes without a chunk load the first one and drop it)
 
     const int kind = p.in_kind;
-    const float inp_scale = kind == kInI32 ? a.inp_scale[PROMPT ? b * p.S + s_query : b] : 0.f;
+    const float inp_scale = kind == kInI32 ? load_uniform(a.inp_scale + (PROMPT ? b * p.S + s_query : b)) : 0.f;
     int rope_row = PROMPT ? (a.rope_row < 0 ? q_pos : a.rope_row + s_query) : (a.rope_row < 0 ? P : a.rope_row);
-    if (!PROMPT && p.rope_rows) rope_row = p.rope_rows[b];
+    if (!PROMPT && p.rope_rows) rope_row = load_uniform(p.rope_rows + b);
     const float *freq = a.freq_cis + (size_t)rope_row * D + e0_in;
     const size_t in_off = PROMPT ? ((size_t)(b * p.S + s_query) * H + h) * D + e0_in : (size_t)bh * D + e0_in;
 
@@ -455,8 +581,8 @@ void kv8_attn_kernel(const Kv8Params p)
     if (has_tail && wave * GPW * UT < n_tail) request_tail(wave * GPW * UT);
     float mask_new = 0.f;
     if (HAS_MASK && appends) mask_new = mrow[P] * kLog2e;
-    float old_weight = 0.f; // of block tid
-    if (gather && direct && tid <= P >> p.t_shift) old_weight = p.weights[(size_t)bh * p.nblk + tid];
+    FirstBlock<D> first_block;
+    if (gather && direct && tid <= P >> p.t_shift) first_block.old = p.weights[(size_t)bh * p.nblk + tid];
     __builtin_amdgcn_sched_barrier(0);
     if (!(appends && fills)) {
         request_scales(r);
@@ -695,13 +821,13 @@ void kv8_attn_kernel(const Kv8Params p)
     if (gather) flush_granules();
 
     // Merge: lane groups in registers, waves through LDS.
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = cross_sum<LPR>(o[i]);
+    scatter_sum<LPR>(o);
     l = cross_sum<LPR>(l);
     lt = cross_sum<LPR>(lt);
-    if (g == 0 && has_chunk) {
+    if ((LPR > 16 || (lane & 15) < LPR) && has_chunk) {
+        const int at = e0 + (LPR <= 32 ? 8 * (lane >> 5) : 0) + (LPR <= 16 ? 4 * (lane >> 4 & 1) : 0);
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4 *>(&s_o[wave][e0 + i]) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        for (int i = 0; i < scattered<LPR>(); i += 4) *reinterpret_cast<float4 *>(&s_o[wave][at + i]) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
     }
     if (lane == 0) {
         s_m[wave] = m;
@@ -741,8 +867,8 @@ void kv8_attn_kernel(const Kv8Params p)
             if (gather) {
                 if (!gran_local) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 __syncthreads(); // every wave's granules are written
-                if (gran_local) add_block_weights<D>(p, bh, P, M, Lsum, tid, [&](int i) __attribute__((always_inline)) { return gran_lds[i]; }, old_weight);
-                else add_block_weights<D>(p, bh, P, M, Lsum, tid, granule_loader(gran_at), old_weight);
+                if (gran_local) add_block_weights<D, false>(p, bh, P, M, Lsum, tid, [&](int i) __attribute__((always_inline)) { return gran_lds[i]; }, first_block);
+                else add_block_weights<D, false>(p, bh, P, M, Lsum, tid, granule_loader(gran_at), first_block);
             }
             return;
         }
@@ -763,9 +889,9 @@ void kv8_attn_kernel(const Kv8Params p)
         }
         __syncthreads();
         if (s_last) {
-            if (gather && tid <= P >> p.t_shift) old_weight = p.weights[(size_t)bh * p.nblk + tid];
-            const float2 ml = combine_partials<D, true>(a, bh, splits, tid, *reinterpret_cast<CombineShared<D> *>(s_merge_bytes));
-            if (gather) add_block_weights<D>(p, bh, P, ml.x, ml.y, tid, granule_loader(gran_at), old_weight);
+            if (gather) first_block.request(p, bh, P, tid, granule_loader(gran_at));
+            const float2 ml = kv8_merge<D, true>(a, bh, splits, tid, *reinterpret_cast<MergeShared<D> *>(s_merge_bytes));
+            if (gather) add_block_weights<D, true>(p, bh, P, ml.x, ml.y, tid, granule_loader(gran_at), first_block);
         }
     }
 }
@@ -774,18 +900,18 @@ void kv8_attn_kernel(const Kv8Params p)
 template <int D>
 __global__ __launch_bounds__(kCombineThreads) void kv8_combine_kernel(const Kv8Params p)
 {
-    __shared__ CombineShared<D> sh;
+    __shared__ MergeShared<D> sh;
     const int bh = blockIdx.x, tid = threadIdx.x, b = bh / p.a.H;
     const int P = p.a.pos_per_seq ? p.a.pos_per_seq[b] : p.a.start_pos;
     if (!kv8_position_ok(p, b, P)) {
         for (int d = tid; d < D; d += kCombineThreads) p.a.out[(size_t)bh * D + d] = __builtin_nanf("");
         return;
     }
-    const float2 ml = combine_partials<D, false>(p.a, bh, kv8_splits(p.a, p.T, P), tid, sh);
-    if (p.weights) {
-        const float old = tid <= P >> p.t_shift ? p.weights[(size_t)bh * p.nblk + tid] : 0.f;
-        add_block_weights<D>(p, bh, P, ml.x, ml.y, tid, granule_loader(p.granules + (size_t)bh * (p.a.L / Kv8Geometry<D>::GR)), old);
-    }
+    const GranuleLoader granule = granule_loader(p.granules + (size_t)bh * (p.a.L / Kv8Geometry<D>::GR));
+    FirstBlock<D> first;
+    if (p.weights) first.request(p, bh, P, tid, granule);
+    const float2 ml = kv8_merge<D, false>(p.a, bh, kv8_splits(p.a, p.T, P), tid, sh);
+    if (p.weights) add_block_weights<D, true>(p, bh, P, ml.x, ml.y, tid, granule, first);
 }
 
 // ---------------------------------------------------------------- prompt phase: append
