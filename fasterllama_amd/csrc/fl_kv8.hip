@@ -229,14 +229,19 @@ hipError_t launch_prompt(const Kv8PromptParams &pp, hipStream_t stream)
         if (!p.stats) return e;
         // Query streams per workgroup of the block weights (see the kernel).  More streams, more and shorter workgroups, but each
         // reads the operands for fewer keys: split until there are four workgroups per compute unit (under a causal mask the
-        // first keys' workgroups see every query, and with two per unit they finish last), not below four query blocks
-        // per stream; a workgroup's 256 / NQ keys are whole blocks.  The whole call, in us, for NQ = 1 / 2 / 4, D = 128:
-        //   32 heads, 4096 queries, all counted  646 / 602 / 621     B=8, 32 heads, 1024, the last 64   234 / 244 / 264
-        //   B=3, 5 heads (D = 96), 333, all       46 / 40 / 37
+        // first keys' workgroups see every query, and with two per unit they finish last), or one where there are only a few
+        // query blocks per stream; a workgroup's 256 / NQ keys are whole blocks.  The whole call, in us, for NQ = 1 / 2 / 4, D = 128:
+        //   32 heads, 4096 queries, all counted  512 / 481 / 473     the last 64   315 / 321 / 334
+        //   B=8, 32 heads, 1024, all             326 / 345 / 393     the last 64   234 / 246 / 270
+        //   8 heads, 2048, all                   161 / 104 /  87     B=3, 5 heads (D = 96), 333, all   47 / 40 / 37
         const int ctx = p.a.start_pos + p.S;
         int NQ = 1;
-        while (NQ < 4 && 2 * NQ * p.T <= 256 && 4 * NQ < pp.kept_blocks && (int64_t)((ctx + 256 / NQ - 1) / (256 / NQ)) * bh < 4 * (int64_t)device_cus()) NQ *= 2;
-        return launch(flattn::kv8_prompt_weights_kernel<D>, dim3((unsigned)((ctx + 256 / NQ - 1) / (256 / NQ)) * bh), block, stream, pp, NQ);
+        while (NQ < 4 && 2 * NQ * p.T <= 256 && NQ < pp.kept_blocks &&
+               (int64_t)((ctx + 256 / NQ - 1) / (256 / NQ)) * bh < (4 * NQ < pp.kept_blocks ? 4 : 1) * (int64_t)device_cus())
+            NQ *= 2;
+        const dim3 weights_grid((unsigned)((ctx + 256 / NQ - 1) / (256 / NQ)) * bh);
+        return NQ == 1 ? launch(flattn::kv8_prompt_weights_kernel<D, true>, weights_grid, block, stream, pp, 1)
+                       : launch(flattn::kv8_prompt_weights_kernel<D, false>, weights_grid, block, stream, pp, NQ);
     }
 }
 
