@@ -267,6 +267,8 @@ __global__ static void kv8_fill_zero_kernel(int32_t *dst, int64_t n)
     if (i < n) dst[i] = 0;
 }
 
+constexpr int64_t kEvictOneLaunchBytes = 128 * 1024; // kept rows of one (b,h), K and V
+
 bool overlap(const void *a, size_t na, const void *b, size_t nb)
 {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
@@ -527,6 +529,13 @@ int fl_kv8_evict(const fl_attn_desc *desc, const fl_kv8_cache *from, const fl_kv
     p.B = desc->batch_size; p.H = desc->head_num; p.D = D; p.T = T; p.t_shift = log2_of(T);
     p.nblk = L / T; p.nblk_to = L_to / T; p.keep = args.keep_blocks; p.recent = args.recent_blocks;
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    // One launch, a workgroup per (b,h), where it has little to move or where there is one for every compute unit; else a
+    // selection, then many workgroups for each.  Two launches / one, us: 15 (b,h) of 96 KB 6.5 / 6.5 and 3 less on the host, 8 of 16 KB
+    // 5.8 / 5.0, 32 of 128 KB 6.8 / 7.4, of 256 KB 9.2 / 12.3, of 512 KB 13.8 / 24.5; 256 of 256 KB 29.4 / 27.6, 2048 208 / 195.
+    if (args.keep_blocks <= flattn::kEvictListCap && ((int64_t)args.keep_blocks * T * D * 2 <= kEvictOneLaunchBytes || (int64_t)bh >= device_cus())) {
+        if (!check_hip(launch(flattn::kv8_evict_kernel, dim3((unsigned)bh), dim3(flattn::kEvictThreads), stream, p))) return FL_ATTN_ERR_HIP;
+        return FL_ATTN_OK;
+    }
     const int slices = (T * D / 16 + 255) / 256;
     if ((int64_t)bh * 2 * slices > INT32_MAX / 128) return FL_ATTN_ERR_SHAPE;
     if (!check_hip(launch(flattn::kv8_select_kernel, dim3((unsigned)bh), dim3(256), stream, p))) return FL_ATTN_ERR_HIP;

@@ -1176,7 +1176,8 @@ __device__ __forceinline__ uint32_t weight_key(float w)
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive prefix sum of a flag over the 256 threads; total: the number of flags set.
+// Exclusive prefix sum of a flag over the NT threads; total: the number of flags set.
+template <int NT>
 __device__ __forceinline__ int block_rank(bool flag, int *s_cnt, int &total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1187,41 +1188,70 @@ __device__ __forceinline__ int block_rank(bool flag, int *s_cnt, int &total)
     int before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NT / 64; ++w) {
         if (w < wave) before += s_cnt[w];
         total += s_cnt[w];
     }
     return before + __popcll(bal & ((1ull << lane) - 1ull));
 }
 
-// grid = B*H, block = 256.  Which blocks stay: the last `recent` and, of the rest, those of the largest weight, ties to the
-// lowest block.  The weight of the last one that stays is found by four passes over the bits of the keys, eight at a time
-// (a histogram in LDS each), so any number of blocks is served; the list is then written in ascending order, and scales and
-// weights move with it.  In place, an entry moves to its own or a lower slot: 256 entries are read before they are written.
-__global__ __launch_bounds__(256) static void kv8_select_kernel(const Kv8EvictParams p)
+// Which blocks of (b,h) stay: the last `recent` and, of the rest, those of the largest weight, ties to the lowest block.  Few
+// candidates count for each how many come before it.  Of many, the weight of the last one that stays is found by four passes over
+// the bits of the keys, eight at a time (a histogram in LDS each).  The list is then written in ascending order, and scales and
+// weights move with it; in place, an entry moves to its own or a lower slot: NT entries are read before they are written.
+constexpr int kCountedBlocks = 64; // (each comes down to 16 reads of four keys)
+struct SelectShared {
+    uint32_t key[kCountedBlocks];
+    int hist[256];
+    int cnt[16];
+    uint32_t pick[2]; // threshold byte, entries still wanted at it
+};
+template <int NT>
+__device__ __forceinline__ void select_blocks(const Kv8EvictParams &p, int bh, int rows, int *s_list, SelectShared &sh)
 {
-    __shared__ int s_hist[256];
-    __shared__ int s_cnt[4];
-    __shared__ uint32_t s_pick[2]; // threshold byte, entries still wanted at it
-    const int bh = blockIdx.x, b = bh / p.H, tid = threadIdx.x;
-    const int rows = evict_rows(p, b);
+    const int b = bh / p.H, tid = threadIdx.x;
     const int n = rows < 0 ? 0 : rows >> p.t_shift;
     const int keep = min(p.keep, n), recent = min(p.recent, keep);
     const int cand = n - recent, want = keep - recent; // the first `cand` blocks compete for `want` places
-    const float *w = p.weights + (size_t)bh * p.nblk;
+    const float *w = p.weights + (size_t)bh * p.nblk, *ks = p.k_scale + (size_t)bh * p.nblk, *vs = p.v_scale + (size_t)bh * p.nblk;
+    const bool all = want >= cand, none = want <= 0, counted = cand <= kCountedBlocks;
+    // the first NT blocks' values, and the open block's
+    float ws = 0.f, ksc = 0.f, vsc = 0.f, w_open = 0.f;
+    if (tid < n) {
+        ws = w[tid];
+        ksc = ks[tid];
+        vsc = vs[tid];
+    }
+    const int open = rows < 0 ? 0 : rows & (p.T - 1);
+    if (tid == 0 && open) w_open = w[n];
     uint32_t prefix = 0, mask = 0;
     int left = want;
-    if (want > 0 && want < cand) {
+    bool chosen = false;
+    if (!all && !none && counted) {
+        if (tid < kCountedBlocks) sh.key[tid] = tid < cand ? weight_key(ws) : 0u;
+        __syncthreads();
+        if (tid < cand) {
+            const uint32_t k = sh.key[tid];
+            int rank = 0;
+#pragma unroll 8
+            for (int i = 0; i < cand; i += 4) { // (keys behind the last are no larger than any, and come later)
+                const uint4 y = *reinterpret_cast<const uint4 *>(&sh.key[i]);
+                rank += (int)(y.x > k || (y.x == k && i < tid)) + (int)(y.y > k || (y.y == k && i + 1 < tid)) +
+                        (int)(y.z > k || (y.z == k && i + 2 < tid)) + (int)(y.w > k || (y.w == k && i + 3 < tid));
+            }
+            chosen = rank < want;
+        }
+    } else if (!all && !none) {
         for (int shift = 24; shift >= 0; shift -= 8) {
-            s_hist[tid] = 0;
+            if (tid < 256) sh.hist[tid] = 0;
             __syncthreads();
-            for (int i = tid; i < cand; i += 256) {
+            for (int i = tid; i < cand; i += NT) {
                 const uint32_t k = weight_key(w[i]);
-                if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255u], 1);
+                if ((k & mask) == prefix) atomicAdd(&sh.hist[(k >> shift) & 255u], 1);
             }
             __syncthreads();
             if (tid < 64) { // the largest byte whose keys and all larger ones are enough: one wave, four bytes a lane
-                const int d3 = s_hist[255 - 4 * tid], d2 = s_hist[254 - 4 * tid], d1 = s_hist[253 - 4 * tid], d0 = s_hist[252 - 4 * tid];
+                const int d3 = sh.hist[255 - 4 * tid], d2 = sh.hist[254 - 4 * tid], d1 = sh.hist[253 - 4 * tid], d0 = sh.hist[252 - 4 * tid];
                 int sum = d3 + d2 + d1 + d0, incl = sum;
 #pragma unroll
                 for (int o = 1; o < 64; o *= 2) {
@@ -1232,88 +1262,123 @@ __global__ __launch_bounds__(256) static void kv8_select_kernel(const Kv8EvictPa
                 if (above < left && incl >= left) {
                     int byte = 255 - 4 * tid, at = above;
                     if (at + d3 < left) { at += d3; --byte; if (at + d2 < left) { at += d2; --byte; if (at + d1 < left) { at += d1; --byte; } } }
-                    s_pick[0] = (uint32_t)byte;
-                    s_pick[1] = (uint32_t)(left - at);
+                    sh.pick[0] = (uint32_t)byte;
+                    sh.pick[1] = (uint32_t)(left - at);
                 }
             }
             __syncthreads();
-            prefix |= s_pick[0] << shift;
+            prefix |= sh.pick[0] << shift;
             mask |= 255u << shift;
-            left = (int)s_pick[1];
+            left = (int)sh.pick[1];
             __syncthreads();
         }
     }
-    // keys above `prefix` stay, and the first `left` equal to it
-    const bool all = want >= cand, none = want <= 0;
     int *list = p.kept + (size_t)bh * p.keep;
     int placed = 0, equal = 0;
-    for (int base = 0; base < n; base += 256) {
+    for (int base = 0; base < n; base += NT) {
         const int i = base + tid;
-        const uint32_t k = i < cand && !all && !none ? weight_key(w[i]) : 0u;
-        const bool tie = i < cand && !all && !none && k == prefix;
-        int n_tie;
-        const int tie_rank = equal + block_rank(tie, s_cnt, n_tie);
-        equal += n_tie;
-        const bool stay = i < n && (i >= cand || all || (!none && (k > prefix || (tie && tie_rank < left))));
-        int n_stay;
-        const int at = placed + block_rank(stay, s_cnt, n_stay);
-        float ws = 0.f, ksc = 0.f, vsc = 0.f;
-        if (stay) {
+        if (base > 0 && i < n) {
             ws = w[i];
-            ksc = p.k_scale[(size_t)bh * p.nblk + i];
-            vsc = p.v_scale[(size_t)bh * p.nblk + i];
+            ksc = ks[i];
+            vsc = vs[i];
         }
-        __syncthreads(); // read before any slot of this trip is written
+        bool stay = i < n && (i >= cand || all);
+        if (!all && !none && counted) {
+            stay = stay || (base == 0 && chosen); // (NT >= kCountedBlocks: every candidate is in the first trip)
+        } else if (!all && !none) { // keys above `prefix` stay, and the first `left` equal to it
+            const uint32_t k = i < cand ? weight_key(ws) : 0u;
+            const bool tie = i < cand && k == prefix;
+            int n_tie;
+            const int tie_rank = equal + block_rank<NT>(tie, sh.cnt, n_tie);
+            equal += n_tie;
+            stay = stay || (i < cand && (k > prefix || (tie && tie_rank < left)));
+        }
+        int n_stay;
+        const int at = placed + block_rank<NT>(stay, sh.cnt, n_stay); // its barriers: read before any slot of this trip is written
         if (stay) {
             list[at] = i;
+            if (s_list) s_list[at] = i;
             p.weights_to[(size_t)bh * p.nblk_to + at] = ws;
             p.k_scale_to[(size_t)bh * p.nblk_to + at] = ksc;
             p.v_scale_to[(size_t)bh * p.nblk_to + at] = vsc;
         }
         placed += n_stay;
     }
-    for (int i = keep + tid; i < p.keep; i += 256) list[i] = -1;
+    for (int i = keep + tid; i < p.keep; i += NT) list[i] = -1;
     if (tid == 0) {
-        const int open = rows < 0 ? 0 : rows & (p.T - 1);
-        if (open && keep < p.nblk_to) p.weights_to[(size_t)bh * p.nblk_to + keep] = w[n]; // the open block's weight
+        if (open && keep < p.nblk_to) p.weights_to[(size_t)bh * p.nblk_to + keep] = w_open;
         if (bh % p.H == 0) p.rows_to[b] = rows < 0 ? -1 : (keep << p.t_shift) + open;
     }
 }
 
-// Moves the listed blocks: grid = B*H * 2 * slices of a block (fastest), block = 256.  A thread owns one 16-byte column of the block for
-// every block it moves, so in place nothing but its own column can stand in its way, and it moves the blocks in ascending
-// order, 8 of them read before the first is written (a block moves to its own or a lower slot).  Bound by the traffic: 1.07 GB
+// Moves one 16-byte column of the listed blocks of K or V.  In place nothing but its own column can stand in its way, and it
+// moves the blocks in ascending order, NB of them read before the first is written (a block moves to its own or a lower slot).
+template <int NB>
+__device__ __forceinline__ void move_column(const Kv8EvictParams &p, int bh, bool is_v, int col, int keep, const int *list)
+{
+    const int cols = p.T * p.D / 16;
+    const u32x4 *src = reinterpret_cast<const u32x4 *>((is_v ? p.v8 : p.k8) + (size_t)bh * p.nblk * p.T * p.D) + col;
+    u32x4 *dst = reinterpret_cast<u32x4 *>((is_v ? p.v8_to : p.k8_to) + (size_t)bh * p.nblk_to * p.T * p.D) + col;
+    for (int r0 = 0; r0 < keep; r0 += NB) {
+        u32x4 x[NB];
+#pragma unroll
+        for (int u = 0; u < NB; ++u) x[u] = __builtin_nontemporal_load(src + (size_t)list[min(r0 + u, keep - 1)] * cols);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < NB; ++u)
+            if (r0 + u < keep) __builtin_nontemporal_store(x[u], dst + (size_t)(r0 + u) * cols);
+    }
+}
+// The open rows of K or V into a cache with tails of its own, by NT threads.
+template <int NT>
+__device__ __forceinline__ void move_tail(const Kv8EvictParams &p, int bh, bool is_v, int rows)
+{
+    _Float16 *tail_to = is_v ? p.v_tail_to : p.k_tail_to;
+    if (!tail_to) return;
+    const half8 *src = reinterpret_cast<const half8 *>((is_v ? p.v_tail : p.k_tail) + (size_t)bh * p.T * p.D);
+    half8 *dst = reinterpret_cast<half8 *>(tail_to + (size_t)bh * p.T * p.D);
+    for (int i = threadIdx.x; i < (rows & (p.T - 1)) * (p.D / 8); i += NT) dst[i] = src[i];
+}
+
+// The selection as a launch of its own: grid = B*H, block = 256.
+__global__ __launch_bounds__(256) static void kv8_select_kernel(const Kv8EvictParams p)
+{
+    __shared__ SelectShared sh;
+    select_blocks<256>(p, blockIdx.x, evict_rows(p, blockIdx.x / p.H), nullptr, sh);
+}
+
+// Moves the listed blocks: grid = B*H * 2 * slices of a block (fastest), block = 256, a thread per column.  Bound by the traffic: 1.07 GB
 // read and written in 195 us, 5.5 TB/s (a plain copy of that size: 5.35; with stores that go through the caches 207 us; 4
 // or 16 blocks at a time 205 / 197).
 __global__ __launch_bounds__(256) static void kv8_move_kernel(const Kv8EvictParams p, int slices)
 {
-    constexpr int NB = 8;
-    const int bh = blockIdx.x / slices >> 1, b = bh / p.H, slice = blockIdx.x % slices;
+    const int bh = blockIdx.x / slices >> 1, slice = blockIdx.x % slices;
     const bool is_v = (blockIdx.x / slices & 1) != 0;
-    const int rows = evict_rows(p, b);
+    const int rows = evict_rows(p, bh / p.H);
     if (rows < 0) return;
-    const int keep = min(p.keep, rows >> p.t_shift);
-    const int col = slice * 256 + threadIdx.x, cols = p.T * p.D / 16;
-    const int *list = p.kept + (size_t)bh * p.keep;
-    if (col < cols) {
-        const u32x4 *src = reinterpret_cast<const u32x4 *>((is_v ? p.v8 : p.k8) + (size_t)bh * p.nblk * p.T * p.D) + col;
-        u32x4 *dst = reinterpret_cast<u32x4 *>((is_v ? p.v8_to : p.k8_to) + (size_t)bh * p.nblk_to * p.T * p.D) + col;
-        for (int r0 = 0; r0 < keep; r0 += NB) {
-            u32x4 x[NB];
-#pragma unroll
-            for (int u = 0; u < NB; ++u) x[u] = __builtin_nontemporal_load(src + (size_t)list[min(r0 + u, keep - 1)] * cols);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int u = 0; u < NB; ++u)
-                if (r0 + u < keep) __builtin_nontemporal_store(x[u], dst + (size_t)(r0 + u) * cols);
-        }
+    const int col = slice * 256 + threadIdx.x;
+    if (col < p.T * p.D / 16) move_column<8>(p, bh, is_v, col, min(p.keep, rows >> p.t_shift), p.kept + (size_t)bh * p.keep);
+    if (slice == 0) move_tail<256>(p, bh, is_v, rows);
+}
+
+// Both in one launch, where a workgroup has little to move: grid = B*H, block = kEvictThreads.
+constexpr int kEvictThreads = 1024, kEvictListCap = 1024;
+__global__ __launch_bounds__(kEvictThreads) static void kv8_evict_kernel(const Kv8EvictParams p)
+{
+    __shared__ SelectShared sh;
+    __shared__ int s_list[kEvictListCap];
+    const int bh = blockIdx.x, rows = evict_rows(p, bh / p.H);
+    select_blocks<kEvictThreads>(p, bh, rows, s_list, sh);
+    if (rows < 0) return; // (uniform)
+    __syncthreads(); // the list
+    const int keep = min(p.keep, rows >> p.t_shift), cols = p.T * p.D / 16;
+    for (int c = threadIdx.x; c < 2 * cols; c += kEvictThreads) {
+        const bool is_v = c >= cols;
+        if (p.keep > 4) move_column<8>(p, bh, is_v, is_v ? c - cols : c, keep, s_list);
+        else move_column<4>(p, bh, is_v, is_v ? c - cols : c, keep, s_list);
     }
-    _Float16 *tail_to = is_v ? p.v_tail_to : p.k_tail_to;
-    if (tail_to && slice == 0) { // the open rows, into a cache with tails of its own
-        const half8 *src = reinterpret_cast<const half8 *>((is_v ? p.v_tail : p.k_tail) + (size_t)bh * p.T * p.D);
-        half8 *dst = reinterpret_cast<half8 *>(tail_to + (size_t)bh * p.T * p.D);
-        for (int i = threadIdx.x; i < (rows & (p.T - 1)) * (p.D / 8); i += 256) dst[i] = src[i];
-    }
+    move_tail<kEvictThreads>(p, bh, false, rows);
+    move_tail<kEvictThreads>(p, bh, true, rows);
 }
 
 } // namespace flattn

@@ -24,6 +24,7 @@ def _need(ok: bool, what: str) -> None:
 # The handle of torch's current stream.  A decode step of a small batch takes less time on the GPU than its call on the host, and
 # building a Stream object for its handle is a sixth of that call; the public way serves where torch lacks the short one.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 class KV8Cache:
@@ -102,7 +103,7 @@ class KV8Attention:
     def _enqueue(self, call, *args) -> None:
         """call(*args, stream) on torch's current stream of this object's device."""
         stream = _raw_stream(self._index)
-        if torch.cuda.current_device() == self._index:
+        if _current_device() == self._index:
             status = call(*args, stream)
         else:
             with torch.cuda.device(self.device):
@@ -154,7 +155,7 @@ class KV8Attention:
             io.q_weight_scale, io.k_weight_scale, io.v_weight_scale = (
                 self._vector(n, t, torch.float32, H * D) for n, t in zip(("q_weight_scale", "k_weight_scale", "v_weight_scale"), scales[1:]))
         if out is None and out_int8 is None:
-            out = torch.empty(out_shape, dtype=torch.float32, device=self.device)
+            out = torch.empty(*out_shape, dtype=torch.float32, device=self.device)  # (a tuple takes 0.3 us longer)
             io.out = out.data_ptr()
         else:
             io.out = None if out is None else self._input("out", out, out_shape, torch.float32)

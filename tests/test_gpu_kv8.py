@@ -1,5 +1,7 @@
 """The 8-bit key/value cache on the GPU, through the C ABI, against float64 (tests/kv8_reference.py).  Rows, scales and tails
 are compared bit for bit, whole arrays, so that a store outside its place shows; what has not been written yet holds NaN."""
+import math
+
 import numpy as np
 import pytest
 
@@ -443,6 +445,31 @@ def test_prompt_over_more_tiles_than_one_list(gpu, kind):
     assert_cache(c.gpu, c.ref, S, start + S)
 
 
+@pytest.mark.parametrize("H", [1, 8])
+def test_block_weights_of_more_queries_than_one_list(gpu, H):
+    """33 000 queries: the list of query blocks is built twice (8 heads: with the operands staged)."""
+    import torch
+    from fasterllama_amd.decode_attn import rope_table
+    from fasterllama_amd.kv8 import KV8Attention, KV8Cache
+    S, L, D, T, W = 33000, 33024, 32, 128, 32990
+    g = torch.Generator(device=gpu).manual_seed(0)
+    q, k, v = (torch.randn(1, S, H, D, generator=g, device=gpu, dtype=torch.float32) for _ in range(3))
+    table, cache = rope_table(L, D, device=gpu), KV8Cache(1, H, D, L, T, weights=True, device=gpu)
+    op = KV8Attention(1, H, D, L, torch.float32, T, max_seq_len=S, device=gpu)
+    op.prefill(q, k, v, cache, table, weight_queries=W)
+    keys, _ = op.read(cache, S)
+    x, f = q[0].double(), table[:S, None].double()
+    rot = torch.stack([x[..., 0::2] * f[..., 0::2] - x[..., 1::2] * f[..., 1::2], x[..., 1::2] * f[..., 0::2] + x[..., 0::2] * f[..., 1::2]], -1).flatten(-2)
+    for h in range(H):
+        want = torch.zeros(L // T * T, dtype=torch.float64, device=gpu)
+        for q0 in range(S - W, S, 2000):
+            z = rot[q0:q0 + 2000, h] @ keys[0, h].double().T / math.sqrt(D)
+            want[:S] += torch.softmax(z, -1).sum(0)
+        want = want.view(-1, T).sum(-1)
+        # every weight is off by its softmax's relative error, a few hundred units of 2^-24 as in assert_cache
+        assert ((cache.weights[0, h].double() - want).abs() <= 2e-5 * want).all()
+
+
 def test_graph_of_a_prompt_an_eviction_and_a_read(gpu):
     """Captured once, replayed with eager work between: every replay equals the eager run."""
     import torch
@@ -586,6 +613,29 @@ def test_evict_many_blocks(gpu):
         want_kept, want_after = kr.evict(c.ref, rows, 700, 100)
         assert np.array_equal(kept.cpu().numpy(), want_kept)
         assert_cache(c.gpu, c.ref)
+
+
+@pytest.mark.parametrize("B,H,D,T,blocks,keep,recent", [
+    (2, 2, 32, 32, 1500, 60, 7),     # one launch, more blocks than its threads, chosen by histograms
+    (16, 16, 128, 128, 7, 5, 1),     # a workgroup for every compute unit
+    (3, 2, 64, 64, 66, 20, 2),       # 64 candidates, counted; two launches
+    (3, 2, 64, 64, 67, 20, 2)])      # 65, by histograms
+@pytest.mark.parametrize("place", ["in place", "other"])
+def test_evict_by_either_way(gpu, B, H, D, T, blocks, keep, recent, place):
+    c = Case(gpu, B, H, D, T * (blocks + 1), T, "f16", 0, weights=True)
+    r = np.random.RandomState(blocks)
+    c.ref.weights[:] = r.randint(0, 9, c.ref.weights.shape)
+    c.ref.k_scale[:], c.ref.v_scale[:] = r.rand(*c.ref.k_scale.shape), r.rand(*c.ref.k_scale.shape)
+    c.ref.k_tail[:], c.ref.v_tail[:] = r.rand(*c.ref.k_tail.shape), r.rand(*c.ref.k_tail.shape)
+    into = None if place == "in place" else kr.Cache(B, H, D, T * (keep + 1), T, True, seed=5)
+    c.gpu, to = to_gpu(c.ref, gpu), None if into is None else to_gpu(into, gpu)
+    rows = T * blocks + 3
+    kept, after = c.op.evict(c.gpu, keep, recent, rows, into=to)
+    want_kept, want_after = kr.evict(c.ref, np.full(B, rows), keep, recent, into)
+    assert np.array_equal(kept.cpu().numpy(), want_kept) and np.array_equal(after.cpu().numpy(), want_after)
+    g, want = (c.gpu, c.ref) if into is None else (to, into)
+    for n in want.names():
+        assert np.array_equal(bits(getattr(g, n).cpu().numpy()), bits(getattr(want, n))), n
 
 
 @pytest.mark.parametrize("T", [32, 64])
