@@ -157,13 +157,11 @@ int check_io(const fl_attn_io *io)
 Kv8Params make_params(const fl_attn_desc *d, const fl_kv8_cache *c, const fl_attn_io *io)
 {
     Kv8Params p{};
-    if (io) {
-        p.a.q = io->q; p.a.k_new = io->k_new; p.a.v_new = io->v_new;
-        p.a.freq_cis = io->freq_cis; p.a.attn_mask = io->attn_mask; p.a.mask_ld = io->mask_ld;
-        p.a.inp_scale = io->qkv_inp_scale; p.a.wq_scale = io->q_weight_scale; p.a.wk_scale = io->k_weight_scale; p.a.wv_scale = io->v_weight_scale;
-        p.a.start_pos = io->start_pos; p.a.rope_row = io->rope_row;
-        p.in_kind = io->qkv_inp_scale ? flattn::kInI32 : (d->dtype == FL_ATTN_F16 ? flattn::kInF16 : flattn::kInF32);
-    }
+    p.a.q = io->q; p.a.k_new = io->k_new; p.a.v_new = io->v_new;
+    p.a.freq_cis = io->freq_cis; p.a.attn_mask = io->attn_mask; p.a.mask_ld = io->mask_ld;
+    p.a.inp_scale = io->qkv_inp_scale; p.a.wq_scale = io->q_weight_scale; p.a.wk_scale = io->k_weight_scale; p.a.wv_scale = io->v_weight_scale;
+    p.a.start_pos = io->start_pos; p.a.rope_row = io->rope_row;
+    p.in_kind = io->qkv_inp_scale ? flattn::kInI32 : (d->dtype == FL_ATTN_F16 ? flattn::kInF16 : flattn::kInF32);
     p.a.B = d->batch_size; p.a.H = d->head_num; p.a.L = d->total_len;
     p.a.scale = d->softmax_scale > 0.f ? d->softmax_scale : 1.0f / sqrtf((float)d->size_per_head);
     p.a.log2_domain = 1;
@@ -458,8 +456,8 @@ int fl_kv8_read(const fl_attn_desc *desc, const fl_kv8_cache *cache, int32_t row
     if (!k_out || !v_out) return FL_ATTN_ERR_NULL_POINTER;
     if (!aligned16(k_out) || !aligned16(v_out) || (reinterpret_cast<uintptr_t>(rows_per_seq) & 3u) != 0) return FL_ATTN_ERR_ALIGNMENT;
     if (rows < 1 || rows > desc->total_len) return FL_ATTN_ERR_POSITION;
-    Kv8Params p = make_params(desc, &c, nullptr);
-    p.a.pos_per_seq = rows_per_seq;
+    const flattn::Kv8ReadParams p = {c.k, c.v, c.k_scale, c.v_scale, static_cast<const _Float16 *>(c.k_tail), static_cast<const _Float16 *>(c.v_tail),
+                                     rows_per_seq, desc->head_num, desc->total_len, c.block_len, log2_of(c.block_len)};
     const int D = desc->size_per_head, vec = desc->dtype == FL_ATTN_F16 ? 8 : 4;
     const int64_t groups = ((int64_t)rows * (D / vec) + 1023) / 1024, grid = groups * 2 * desc->batch_size * desc->head_num;
     if (grid > INT32_MAX / 128) return FL_ATTN_ERR_SHAPE; // 2^32 threads a launch

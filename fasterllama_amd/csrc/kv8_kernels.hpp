@@ -1080,19 +1080,26 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(const Kv8Params p)
 // out_k, out_v [B,H,n,D] in O: integers * scale for complete blocks, the tail behind them, zeros behind a sequence's rows.
 // grid = B*H * 2 * groups (the groups of 1024 chunks of one (b,h) fastest), block = 256; a lane writes 16 bytes.  Bound by the traffic, D bytes in and
 // D * sizeof(O) out per row: 201 MB in 33 us, 6.2 TB/s.
+struct Kv8ReadParams { // (a launch copies its arguments to the device: a third of Kv8Params is 0.2 us less)
+    const int8_t *k8, *v8;
+    const float *k_scale, *v_scale;
+    const _Float16 *k_tail, *v_tail;
+    const int32_t *rows_per_seq; // [B] or NULL
+    int32_t H, L, T, t_shift;
+};
 template <typename O>
-__global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8Params p, O *out_k, O *out_v, int n, int D, int groups)
+__global__ __launch_bounds__(256) void kv8_read_kernel(const Kv8ReadParams p, O *out_k, O *out_v, int n, int D, int groups)
 {
     constexpr int VEC = 16 / (int)sizeof(O), NU = 4;
     typedef O vec __attribute__((ext_vector_type(VEC)));
-    const int bh = blockIdx.x / groups >> 1, b = bh / p.a.H;
+    const int bh = blockIdx.x / groups >> 1, b = bh / p.H;
     const bool is_v = (blockIdx.x / groups & 1) != 0;
     // rows in the cache (a negative count: all zeros): where they end, not where the output does, the tail begins
-    const int rows = min(p.a.pos_per_seq ? p.a.pos_per_seq[b] : n, p.a.L);
+    const int rows = min(p.rows_per_seq ? p.rows_per_seq[b] : n, p.L);
     const int rows8 = rows > 0 ? rows & ~(p.T - 1) : 0;
-    const int8_t *src = (is_v ? p.v8 : p.k8) + (size_t)bh * p.a.L * D;
+    const int8_t *src = (is_v ? p.v8 : p.k8) + (size_t)bh * p.L * D;
     const _Float16 *tail = (is_v ? p.v_tail : p.k_tail) + (size_t)bh * p.T * D;
-    const float *scale = (is_v ? p.v_scale : p.k_scale) + (size_t)bh * p.nblk;
+    const float *scale = (is_v ? p.v_scale : p.k_scale) + (size_t)bh * (p.L >> p.t_shift);
     O *out = (is_v ? out_v : out_k) + (size_t)bh * n * D;
     const uint32_t CPR = D / VEC, total = (uint32_t)n * CPR; // (n * D stays below 2^31)
     const uint32_t i0 = (blockIdx.x % groups) * (256 * NU) + threadIdx.x;

@@ -134,7 +134,13 @@ class KV8Attention:
         B, H, _, D = self.shape
         io, shape = self.io, (B, seq_len, H, D)
         dtype = self.dtype if scales is None else torch.int32
-        io.q, io.k_new, io.v_new = self._input("q", q, shape, dtype), self._input("k_new", k_new, shape, dtype), self._input("v_new", v_new, shape, dtype)
+        index = self._index
+        if (q.dtype is not dtype or k_new.dtype is not dtype or v_new.dtype is not dtype or q.shape != shape or k_new.shape != shape
+                or v_new.shape != shape or not q.is_contiguous() or not k_new.is_contiguous() or not v_new.is_contiguous()
+                or q.get_device() != index or k_new.get_device() != index or v_new.get_device() != index):
+            for name, t in (("q", q), ("k_new", k_new), ("v_new", v_new)):  # which one
+                self._input(name, t, shape, dtype)
+        io.q, io.k_new, io.v_new = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr()
         rows = freq_cis.shape[0]
         if rows < rope_rows:
             _need(False, f"freq_cis has {rows} rows, the call uses {rope_rows}")
@@ -159,8 +165,8 @@ class KV8Attention:
             io.out = out.data_ptr()
         else:
             io.out = None if out is None else self._input("out", out, out_shape, torch.float32)
-        io.out_int8 = self._vector("out_int8", out_int8, torch.int8, B * seq_len * H * D)
-        io.out_scale = self._vector("out_scale", out_scale, torch.float32, B * seq_len)
+        io.out_int8 = None if out_int8 is None else self._vector("out_int8", out_int8, torch.int8, B * seq_len * H * D)
+        io.out_scale = None if out_scale is None else self._vector("out_scale", out_scale, torch.float32, B * seq_len)
         return out
 
     def decode(self, q, k_new, v_new, cache: KV8Cache, freq_cis, start_pos: int = 0, attn_mask=None, start_pos_per_seq=None,
@@ -177,11 +183,11 @@ class KV8Attention:
         rope_rows = 0 if rope_row_per_seq is not None else (last if rope_row < 0 else rope_row) + 1
         out = self._fill(q, k_new, v_new, 1, freq_cis, rope_rows, attn_mask, last, scales, out, (B, H * D), out_int8, out_scale)
         io = self.io
-        io.start_pos_per_seq = self._vector("start_pos_per_seq", start_pos_per_seq, torch.int32, B)
+        io.start_pos_per_seq = None if start_pos_per_seq is None else self._vector("start_pos_per_seq", start_pos_per_seq, torch.int32, B)
         io.start_pos, io.max_start_pos, io.rope_row = start_pos, max_start_pos, rope_row
         io.flags = capi.FL_ATTN_IO_WORKSPACE_READY
         self._enqueue(self.lib.fl_kv8_decode_forward, self._desc, cache.ref, self._io,
-                      self._vector("rope_row_per_seq", rope_row_per_seq, torch.int32, B), freq_cis.shape[0])
+                      None if rope_row_per_seq is None else self._vector("rope_row_per_seq", rope_row_per_seq, torch.int32, B), freq_cis.shape[0])
         return out
 
     def prefill(self, q, k_new, v_new, cache: KV8Cache, freq_cis, start_pos: int = 0, attn_mask=None, mask_tile_classes=None,
