@@ -433,7 +433,8 @@ __device__ __forceinline__ int kv8_splits(const Params &a, int T, int P) { retur
 // flight, at no register's cost; the first trip is requested before the query has arrived.  B=64, 32 heads, D = 128, 2041
 // rows, mask and weights: 169 us for 1.104 GB (counted: 1.103), 6.5 TB/s of the 7.1 that two streams of plain reads reach;
 // without any arithmetic the same loads take as long.  Three waves per SIMD: a fourth (128 registers) changes nothing where
-// it does not spill, and costs a quarter of the time where it does.  One long sequence (32 heads, 4083 rows, 9 splits): 13 us.
+// it does not spill, and costs a quarter of the time where it does.  One long sequence (32 heads, 4083 rows, 9 splits): 12 us, 7
+// behind the streaming and before it.
 template <int D, bool HAS_MASK, bool PROMPT>
 __global__ __launch_bounds__(kKv8Waves * 64) __attribute__((amdgpu_waves_per_eu(D > 512 ? 2 : 3, 8)))
 void kv8_attn_kernel(const Kv8Params p)
@@ -1354,9 +1355,8 @@ __global__ __launch_bounds__(256) static void kv8_select_kernel(const Kv8EvictPa
     select_blocks<256>(p, blockIdx.x, evict_rows(p, blockIdx.x / p.H), nullptr, sh);
 }
 
-// Moves the listed blocks: grid = B*H * 2 * slices of a block (fastest), block = 256, a thread per column.  Bound by the traffic: 1.07 GB
-// read and written in 195 us, 5.5 TB/s (a plain copy of that size: 5.35; with stores that go through the caches 207 us; 4
-// or 16 blocks at a time 205 / 197).
+// Moves the listed blocks: grid = B*H * 2 * slices of a block (fastest), block = 256, a thread per column.  32 (b,h) of 512 KB: 14 us
+// with the selection.
 __global__ __launch_bounds__(256) static void kv8_move_kernel(const Kv8EvictParams p, int slices)
 {
     const int bh = blockIdx.x / slices >> 1, slice = blockIdx.x % slices;
@@ -1368,7 +1368,9 @@ __global__ __launch_bounds__(256) static void kv8_move_kernel(const Kv8EvictPara
     if (slice == 0) move_tail<256>(p, bh, is_v, rows);
 }
 
-// Both in one launch, where a workgroup has little to move: grid = B*H, block = kEvictThreads.
+// Both in one launch, where a workgroup has little to move or there is one for every compute unit: grid = B*H, block = kEvictThreads.
+// Bound by the traffic: 1.07 GB read and written in 190 us, 5.6 TB/s (a plain copy of half of that: 5.35; in two launches 200,
+// there with stores that go through the caches 212, with 4 or 16 blocks at a time 210 / 202).
 constexpr int kEvictThreads = 1024, kEvictListCap = 1024;
 __global__ __launch_bounds__(kEvictThreads) static void kv8_evict_kernel(const Kv8EvictParams p)
 {
