@@ -188,9 +188,7 @@ template <int D>
 hipError_t launch_append(const Kv8Params &p, hipStream_t stream)
 {
     const int n = (p.a.start_pos + p.S) / p.T - p.a.start_pos / p.T;
-    const int64_t groups = (int64_t)p.a.B * p.a.H * 2 * (n > 0 ? n : 1);
-    if (groups > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)groups), block(256);
+    const dim3 grid((unsigned)(p.a.B * p.a.H * 2 * (n > 0 ? n : 1))), block(256);
     if (p.T == 32) return launch(flattn::kv8_append_kernel<D, 32>, grid, block, stream, p);
     if (p.T == 64) return launch(flattn::kv8_append_kernel<D, 64>, grid, block, stream, p);
     return launch(flattn::kv8_append_kernel<D, 128>, grid, block, stream, p);
@@ -397,10 +395,13 @@ int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, 
     if (seq_len < 1 || io.start_pos < 0 || (int64_t)io.start_pos + seq_len > L) return FL_ATTN_ERR_POSITION;
     if (io.attn_mask && (io.mask_ld < 0 || (io.mask_ld != 0 && io.mask_ld < (int64_t)io.start_pos + seq_len))) return FL_ATTN_ERR_ARGUMENT;
     if (c.weights && D > 128) return FL_ATTN_ERR_HEAD_DIM;
-    // A workgroup per query and head where the head size is beyond 128, of the 2^32 threads a launch may have; the mask's
-    // classes are a two-dimensional grid.
+    // A launch has fewer than 2^32 threads: two workgroups per head and block that is filled, one per query and head where the head
+    // size is beyond 128, one per token for INT8 output; the mask's classes are a two-dimensional grid.
     const int64_t queries = (int64_t)desc->batch_size * desc->head_num * seq_len;
-    if (queries > (int64_t)INT32_MAX || (D > 128 && queries * flattn::kKv8Waves * 64 > (int64_t)UINT32_MAX) ||
+    const int64_t filled = (io.start_pos + seq_len) / c.block_len - io.start_pos / c.block_len;
+    if (queries > (int64_t)INT32_MAX || (int64_t)desc->batch_size * desc->head_num * 2 * filled > (int64_t)(UINT32_MAX / 256) ||
+        (D > 128 && queries > (int64_t)(UINT32_MAX / (flattn::kKv8Waves * 64))) ||
+        (io.out_int8 && (int64_t)desc->batch_size * seq_len > (int64_t)(UINT32_MAX / flattn::kQuantThreads)) ||
         seq_len > 65535 * flattn::kPrefillQueriesPerBlock)
         return FL_ATTN_ERR_SHAPE;
     const Layout w = layout(desc, seq_len);

@@ -111,6 +111,11 @@ def test_decode_only_and_prompt_only():
     assert prefill(d=desc(D=256)) == capi.FL_ATTN_ERR_HEAD_DIM  # weights beyond 128
     wide = desc(B=64, H=64, D=256, L=8192)  # a workgroup per query: 2^32 threads
     assert prefill(d=wide, c=fake_cache(weights=None), io=fake_io(start_pos=0), S=4096) == capi.FL_ATTN_ERR_SHAPE
+    many = desc(B=1024, H=64, D=32, L=8192)  # blocks to fill
+    assert prefill(d=many, c=fake_cache(weights=None), io=fake_io(start_pos=0), S=8192) == capi.FL_ATTN_ERR_SHAPE
+    tokens = desc(B=4096, H=1, D=32, L=4096)  # tokens to quantise
+    io = fake_io(start_pos=0, out_int8=0x1000, out_scale=0x1000)
+    assert prefill(d=tokens, c=fake_cache(weights=None), io=io, S=4096) == capi.FL_ATTN_ERR_SHAPE
     n = C.c_size_t()
     assert capi.load().fl_kv8_workspace_bytes(C.byref(desc()), 64, 257, C.byref(n)) == capi.FL_ATTN_ERR_POSITION
 
