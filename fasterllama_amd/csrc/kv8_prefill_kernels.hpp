@@ -5,8 +5,9 @@
 // What the 8 bits change:
 //   operands   a byte is an exact fp16 number, so K and V enter v_mfma_f32_32x32x16_f16 as they are stored and the block's
 //              scale (uniform over a 32-key tile) stays outside: K's multiplies the score where the softmax scale does, V's
-//              goes into the exponent of the weight, e^(s - m) * vs / vref = 2^(s' - m' + log2(vs / vref)), and costs nothing
-//              per score either;
+//              goes into the exponent of the weight, e^(s - m) * vs / 2^r = 2^(s' - m' + log2(vs) - r), and costs nothing
+//              per score either.  A query's references m and r follow the largest PRODUCT of weight and scale met so far: a
+//              block of large values that gets no weight, or one of zeros, must not decide how finely the others' are held;
 //   precision  queries and weights are fp16 PAIRS, value + remainder (22 bits), twice the matrix instructions of single
 //              values, so that the output keeps the accuracy of 32-bit arithmetic (2e-7 of the result at the 7B shapes;
 //              weights rounded once to fp16 would leave 1.4e-4).  A query is scaled by a power of two so that its largest
@@ -25,9 +26,10 @@
 
 namespace flattn {
 
-// Weights enter the second product times the block's share vs / vref of the largest V scale so far: what a block 2^30 below it
-// adds is lost in the remainder's smallest step, 2^-31 of the largest value.
-constexpr float kKv8WeightExp = 7.0f; // weights enter the second product times 2^7; kLazyMax = 8 more stay below 65504
+// Weights times V scale enter the second product relative to a query's largest such product, times 2^7; kLazyMax = 8 more stay below
+// 65504.  The remainder's smallest step is 2^-24: a weight is held to 2^-22 of itself or to 2^-32 of that largest product.
+constexpr float kKv8WeightExp = 7.0f;
+constexpr int kKv8LeastScaleExp = -40; // a block's scale is 0 or at least 2^-31 (fp16's smallest step over 127): 0 counts as 2^-40
 
 struct Kv8PromptParams {
     Kv8Params k;
@@ -341,8 +343,8 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
         for (int v = 0; v < 16; ++v) ot[dt][v] = 0.f;
-    float m = kMaxFloor * kLog2e, l = 0.f;
-    uint32_t vref = 0u; // bits of the power of two that the output accumulators are in units of (uniform); 0: none yet
+    // Per query: weights are 2^(s' - m), l is their sum, output accumulators are in units of 2^r (a whole number).
+    float m = kMaxFloor * kLog2e, r = (float)kKv8LeastScaleExp, l = 0.f;
     const int vrow = 4 * hf + ((lane & 15) >> 2), vcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
     for (int c = 0; c < NC; ++c) asm volatile("" : "+v"(qhi[c]), "+v"(qlo[c]));
@@ -431,28 +433,23 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
                     }
                     cs = 1.f;
                 }
-                // The accumulators' unit: a power of two no smaller than any block's scale so far.
-                const float vs = vs_tile == 0.f ? 1.f : vs_tile; // a block of zeros
-                const uint32_t vbits = __builtin_amdgcn_readfirstlane((__float_as_uint(vs) + 0x7fffffu) & 0xff800000u);
-                if (vbits > vref) { // uniform
-                    const float down = __uint_as_float(vref) * __uint_as_float(0x7f000000u - vbits); // (reciprocal of a power of two)
-                    vref = vbits;
-#pragma unroll
-                    for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                        for (int v = 0; v < 16; ++v) ot[dt][v] *= down;
-                }
-                const float lr = __builtin_amdgcn_logf(vs * __uint_as_float(0x7f000000u - vref)) + kKv8WeightExp; // log2
-                const float mx = fmaxf(m, cross_half_max(max16(st)) * cs);
-                if (__ballot(mx > m + kLazyMax) != 0ull) { // wave-uniform
-                    const float alpha = __builtin_amdgcn_exp2f(m - mx);
-                    m = mx;
-                    l *= alpha;
+                // log2 of the block's scale as a whole number and a fraction, so that its differences to r stay exact
+                const uint32_t vbits = __builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(vs_tile, __builtin_ldexpf(1.0f, kKv8LeastScaleExp))));
+                const float vexp = (float)((int)(vbits >> 23) - 127), vfrac = __builtin_amdgcn_logf(__uint_as_float((vbits & 0x7fffffu) | 0x3f800000u));
+                const float mx = cross_half_max(max16(st)) * cs;
+                const float over = (mx - m) + (vexp - r) + vfrac; // of this tile's largest product over the reference (-inf: all masked)
+                if (__ballot(over > kLazyMax) != 0ull) { // wave-uniform
+                    const float m_new = over > 0.f ? mx : m, r_new = over > 0.f ? vexp : r; // (what l counts stays within 2^57 of 1)
+                    const float alpha = __builtin_amdgcn_exp2f((m - m_new) + (r - r_new));
+                    l *= __builtin_amdgcn_exp2f(m - m_new);
+                    m = m_new;
+                    r = r_new;
 #pragma unroll
                     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
                         for (int v = 0; v < 16; ++v) ot[dt][v] *= alpha;
                 }
+                const float lr = (vexp - r) + vfrac + kKv8WeightExp;
                 const float nb = lr - m;
                 half8 ph[2], pl[2];
                 float sum0 = 0.f, sum1 = 0.f;
@@ -505,8 +502,8 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
         if (KS > 1) pp.part_ml[slot * pp.part_rows + wave * 32 + qi] = make_float2(m, l);
         else if (p.stats) p.stats[(size_t)bh * S + q_row] = make_float2(m, l);
     }
-    // e^(..) sums to l, accumulators are in units of vref with weights times 2^7; a fully masked query: 0 / 0
-    const float rl = __uint_as_float(vref) * (1.0f / 128.0f) / (KS > 1 ? 1.0f : l);
+    // e^(..) sums to l, accumulators are in units of 2^r with weights times 2^7; a fully masked query: 0 / 0
+    const float rl = __builtin_ldexpf(1.0f, (int)(r - kKv8WeightExp)) / (KS > 1 ? 1.0f : l);
     __syncthreads(); // every wave is done with the last tile
     float *so = reinterpret_cast<float *>(smem) + wave * 32 * LDO;
     const int q0 = qb * kPrefillQueriesPerBlock + wave * 32;

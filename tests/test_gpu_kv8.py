@@ -732,3 +732,93 @@ def test_caches_past_four_gib(gpu):
         assert_out(got[[b]], want[:, :, 0].reshape(1, D), tol.reshape(1, 1))
         assert np.array_equal(cache.k[b, 0, -128:].cpu().numpy(), small.k[0, 0, 128:])
     assert np.isnan(got[1:B - 1].cpu().numpy()).all()
+
+
+# ----------------------------------------------------------------------------------------- values of very different sizes
+
+def weighted_tolerance(c, q_rot, P, S, mask):
+    """Per query [B,H,S,1], from the reference's state after the call: the 32-bit bound of Cache.tolerance(), relative to what the
+    query weighs instead of to the largest |v| of the cache: the larger of max_d sum_j p_j |v_jd| and max_j p_j (absmax of j's block).
+    A kernel that holds a weight to 2^-32 of the largest product of weight and block scale adds rows * 2^-32 of the second: 16 U at 4096."""
+    ref, T, out = c.ref, c.T, []
+    scale = c.scale or 1.0 / math.sqrt(c.D)
+    for b in range(c.B):
+        k, v = ref.values(b, P + S)
+        z = q_rot[b] @ k.transpose(0, 2, 1) * scale
+        with np.errstate(invalid="ignore", over="ignore"):
+            if mask is not None:
+                z = z + mask[P:P + S, :P + S].astype(np.float64)
+            e = np.exp(z - np.maximum(z.max(-1, keepdims=True), -1e9))
+            p = e / e.sum(-1, keepdims=True)
+        n = P + S
+        block = np.abs(np.pad(v, ((0, 0), (0, -n % T), (0, 0)))).reshape(c.H, -1, T * c.D).max(-1).repeat(T, -1)[:, :n]
+        weighs = np.maximum((p @ np.abs(v)).max(-1), (p * block[:, None]).max(-1))
+        A = scale * np.abs(q_rot[b]).max() * np.abs(k).sum(-1).max()
+        out.append(kr.U * (4 * A + math.sqrt(n) + 64) * weighs[..., None])
+    return np.stack(out)
+
+
+def prompt_of(c, q, k, v, m, **kw):
+    """A prompt of the given float32 inputs [B,S,H,D]: (out, expected, tolerance per query)."""
+    P, S = int(c.rows[0]), q.shape[1]
+    got = c.op.prefill(c.t(q), c.t(k), c.t(v), c.gpu, c.table_d, start_pos=P, attn_mask=c.t(m), **kw)
+    want, _ = c.ref.step(q, k, v, c.table, c.rows, m, None, c.scale)
+    return got, want, weighted_tolerance(c, kr.rotate(q, c.table[P:P + S][:, None]).transpose(0, 2, 1, 3), P, S, m)
+
+
+@pytest.mark.parametrize("kind", [None, "causal"])
+@pytest.mark.parametrize("amp", [1.0, 1e-3, 1e-5])
+@pytest.mark.parametrize("D,T,S", [(128, 64, 320), (64, 32, 96), (96, 128, 384), (32, 32, 1024), (256, 64, 128)])
+def test_values_behind_a_block_of_zeros(gpu, D, T, S, amp, kind):
+    """Padding is zeros: a block with no scale says nothing about the size of the values that follow it."""
+    c = Case(gpu, 1, 2, D, S + T, T, "f32", 0, max_seq_len=S, weights=D <= 128)
+    _, val, _ = c.feed(S, 3)
+    q, k, v = (x.copy() for x in val)
+    k[:, :T] = 0
+    v[:, :T] = 0
+    v *= np.float32(amp)
+    m = masks(kind, S + T)
+    got, want, tol = prompt_of(c, q, k, v, m)
+    if kind:
+        assert not got[:, :, :T].cpu().numpy().any()  # queries that see zeros only
+    assert_out(got, want, tol, f"amp {amp}")
+    assert_cache(c.gpu, c.ref, S, S)
+    kk, vv = c.op.read(c.gpu, S)
+    for x, y in zip((kk, vv), c.ref.values(0, S)):
+        assert np.array_equal(x[0].cpu().numpy(), y.astype(np.float32))
+    # and a step behind them
+    c.rows[:] = S
+    _, val, _ = c.feed(1, 4)
+    q1, k1, v1 = (x.copy() for x in val)
+    v1 *= np.float32(amp)
+    got = c.op.decode(c.t(q1), c.t(k1), c.t(v1), c.gpu, c.table_d, start_pos=S)
+    want, _ = c.ref.step(q1, k1, v1, c.table, c.rows)
+    tol = weighted_tolerance(c, kr.rotate(q1, c.table[S:S + 1][:, None]).transpose(0, 2, 1, 3), S, 1, None)
+    assert_out(got, want[:, :, 0], tol[:, :, 0], "step")
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** 10, 2.0 ** 14, 2.0 ** 18])
+@pytest.mark.parametrize("large", ["first", "last"])
+@pytest.mark.parametrize("D,T,start", [(128, 64, 0), (64, 32, 0), (32, 128, 0), (128, 64, 1280)])
+def test_large_values_of_little_weight_leave_the_others_precision(gpu, D, T, start, large, ratio):
+    """A block of large values with scores 20 lower, before or behind small ones that get nearly all of the weight (`start`: the
+    keys are shared by several workgroups)."""
+    S = 4 * T if start == 0 else 64
+    L = start + S
+    c = Case(gpu, 1, 2, D, L, T, "f32", 0, max_seq_len=S if start == 0 else 256)
+    _, val, _ = c.feed(L, 5)
+    q, k, v = (x.copy() for x in val)
+    at = slice(0, T) if large == "first" else slice(L - T, L)
+    small = np.ones((1, L, 1, 1), np.float32) / np.float32(ratio)
+    small[:, at] = 1
+    v *= small
+    m = np.zeros((L, L), np.float32)
+    m[:, at] = -20
+    for P in range(0, start, 256):  # what lies before the piece that is looked at
+        n = min(256, start - P)
+        c.rows[:] = P
+        c.op.prefill(*(c.t(x[:, P:P + n]) for x in (q, k, v)), c.gpu, c.table_d, start_pos=P, attn_mask=c.t(m))
+        c.ref.step(*(x[:, P:P + n] for x in (q, k, v)), c.table, c.rows, m)
+    c.rows[:] = start
+    got, want, tol = prompt_of(c, q[:, start:], k[:, start:], v[:, start:], m)
+    assert_out(got, want, tol, f"ratio {ratio}")
