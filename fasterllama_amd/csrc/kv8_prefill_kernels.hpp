@@ -450,7 +450,12 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
                         for (int v = 0; v < 16; ++v) ot[dt][v] *= alpha;
                 }
                 const float lr = (vexp - r) + vfrac + kKv8WeightExp;
-                const float nb = lr - m;
+                float nb = lr - m;
+                if (special) { // next to a mask's -1e9 the scale's share would be rounded away: the difference first
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) st[v] -= m;
+                    nb = lr;
+                }
                 half8 ph[2], pl[2];
                 float sum0 = 0.f, sum1 = 0.f;
                 float minus1 = -1.0f; // opaque, so that e - h stays one mixed-precision FMA instead of a conversion and a subtraction

@@ -822,3 +822,60 @@ def test_large_values_of_little_weight_leave_the_others_precision(gpu, D, T, sta
     c.rows[:] = start
     got, want, tol = prompt_of(c, q[:, start:], k[:, start:], v[:, start:], m)
     assert_out(got, want, tol, f"ratio {ratio}")
+
+
+@pytest.mark.parametrize("kind", [None, "causal"])
+@pytest.mark.parametrize("amp", [1e4, 1e-3, 1e-5])
+@pytest.mark.parametrize("D,T,start,S", [(128, 64, 0, 300), (64, 128, 77, 150), (96, 32, 13, 60), (32, 64, 0, 40), (128, 64, 1300, 40), (256, 64, 5, 100)])
+def test_small_and_large_values_in_the_open_block(gpu, D, T, start, S, amp, kind):
+    """Rows of the open block are values, with no scale beside them; the blocks before them are integers of a scale."""
+    L = -(-(start + S) // T) * T
+    c = Case(gpu, 1, 2, D, L, T, "f32", 0, max_seq_len=max(S, 256) if L >= 256 else L)
+    _, val, _ = c.feed(start + S, 5)
+    q, k, v = (x.copy() for x in val)
+    v *= np.float32(amp)
+    m = masks(kind, L)
+    for P in range(0, start, 256):
+        n = min(256, start - P)
+        c.rows[:] = P
+        c.op.prefill(*(c.t(x[:, P:P + n]) for x in (q, k, v)), c.gpu, c.table_d, start_pos=P, attn_mask=c.t(m))
+        c.ref.step(*(x[:, P:P + n] for x in (q, k, v)), c.table, c.rows, m)
+    c.rows[:] = start
+    got, want, tol = prompt_of(c, q[:, start:], k[:, start:], v[:, start:], m)
+    assert_out(got, want, tol, f"amp {amp}")
+    assert_cache(c.gpu, c.ref, S, start + S)
+
+
+@pytest.mark.parametrize("D,T,start,S", [(128, 64, 0, 320), (64, 32, 77, 150), (96, 128, 0, 300), (32, 32, 0, 64), (128, 64, 1300, 40), (256, 64, 0, 128)])
+def test_rows_masked_by_a_finite_value_weigh_their_keys_evenly(gpu, D, T, start, S):
+    """-1e9 on every key of a row: next to it a score is less than half a step of a 32-bit float, so all keys weigh the same, as in
+    the caches of the other types; the blocks' scales differ."""
+    L = -(-(start + S) // T) * T
+    c = Case(gpu, 1, 2, D, L, T, "f32", 0, max_seq_len=max(S, 256) if L >= 256 else L)
+    _, val, _ = c.feed(start + S, 6)
+    q, k, v = (x.copy() for x in val)
+    r = np.random.RandomState(0)
+    v *= np.exp2(r.randint(-8, 9, (1, -(-(start + S) // T), 1, 1))).astype(np.float32).repeat(T, 1)[:, :start + S]
+    m = masks("causal", L)
+    m[start + 3:start + 40:3] = -1e9
+    for P in range(0, start, 256):
+        n = min(256, start - P)
+        c.rows[:] = P
+        c.op.prefill(*(c.t(x[:, P:P + n]) for x in (q, k, v)), c.gpu, c.table_d, start_pos=P, attn_mask=c.t(m))
+        c.ref.step(*(x[:, P:P + n] for x in (q, k, v)), c.table, c.rows, m)
+    c.rows[:] = start
+    got, want, tol = prompt_of(c, q[:, start:], k[:, start:], v[:, start:], m)
+    n = start + S
+    _, vv = c.ref.values(0, n)
+    for s in range(3, min(S, 40), 3):
+        want[0, :, s] = vv.mean(1)
+        # n equal weights: the sums' and the quotient's roundings, of the mean |v| (largest over the elements)
+        tol[0, :, s] = kr.U * (math.sqrt(n) + 64) * np.abs(vv).mean(1).max(-1, keepdims=True)
+    assert_out(got, want, tol)
+    # the decode step under such a row
+    if n < L:
+        c.rows[:] = n
+        m[n] = -1e9
+        got, want, _ = c.decode(m)
+        _, vv = c.ref.values(0, n + 1)
+        assert_out(got, vv.mean(1)[None], kr.U * (math.sqrt(n) + 64) * np.abs(vv).mean(1).max(-1)[None, :, None], "step")
