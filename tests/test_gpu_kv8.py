@@ -879,3 +879,49 @@ def test_rows_masked_by_a_finite_value_weigh_their_keys_evenly(gpu, D, T, start,
         got, want, _ = c.decode(m)
         _, vv = c.ref.values(0, n + 1)
         assert_out(got, vv.mean(1)[None], kr.U * (math.sqrt(n) + 64) * np.abs(vv).mean(1).max(-1)[None, :, None], "step")
+
+
+# ------------------------------------------------------------------------------------------- long contexts of one workgroup
+
+def long_case(dev, D, T, rows, L, weights=True, **kw):
+    """A cache of `rows` rows without the reference's row by row filling: random bytes, neighbouring blocks of different scales."""
+    c = Case(dev, 1, 1, D, L, T, "f16", 0, weights=weights, **kw)
+    r, n = np.random.RandomState(D + rows), L // T
+    c.ref.k_scale[:], c.ref.v_scale[:] = 0.02 * np.exp2(r.randint(-2, 2, (1, 1, n))), 0.02 * np.exp2(r.randint(-3, 3, (1, 1, n)))
+    c.ref.k_tail[:], c.ref.v_tail[:] = r.randn(*c.ref.k_tail.shape), r.randn(*c.ref.k_tail.shape)
+    if weights:
+        c.ref.weights[:] = r.rand(*c.ref.weights.shape)
+    c.gpu, c.rows = to_gpu(c.ref, dev), np.array([rows])
+    return c
+
+
+@pytest.mark.parametrize("D,T,rows", [(1024, 32, 1100), (1024, 64, 2111), (1024, 128, 4200), (512, 64, 2200), (256, 32, 4190), (256, 128, 16500),
+                                      (128, 64, 8300), (96, 32, 8254), (64, 32, 8319), (32, 128, 8250), (128, 128, 33000)])
+@pytest.mark.parametrize("kind", [None, "causal"])
+def test_one_workgroup_walks_a_long_context(gpu, D, T, rows, kind):
+    """nsplit = 1: more rows than the lanes of a wave hold scales and granules for, and than granules fit beside the merge; two steps,
+    of which one may fill a block."""
+    L = (rows // T + 2) * T
+    c = long_case(gpu, D, T, rows, L, nsplit=1)
+    for step in range(2):
+        c.rows[:] = rows + step
+        m = None
+        if kind:  # one row for every position: the last 100 keys and every seventh are hidden
+            m = np.zeros((1, L), np.float32)
+            m[0, rows - 100:] = NEG
+            m[0, ::7] = -np.inf
+            m[0, rows:] = 0
+        raw, val, _ = c.feed(1, 20 + step)
+        got = c.op.decode(*raw, c.gpu, c.table_d, start_pos=rows + step, attn_mask=c.t(m))
+        want, tol = c.ref.step(*val, c.table, c.rows, None if m is None else np.broadcast_to(m, (L, L)))
+        assert_out(got, want[:, :, 0], tol[..., 0], f"step {step}")
+    assert_cache(c.gpu, c.ref, 2)
+
+
+@pytest.mark.parametrize("D,T,start", [(1024, 32, 1100), (512, 128, 2300), (256, 64, 4200)])
+def test_wide_prompt_behind_a_long_context(gpu, D, T, start):
+    S, L = 5, (start // T + 2) * T
+    c = long_case(gpu, D, T, start, L, weights=False, max_seq_len=S)
+    got, want, tol = c.prompt(S, masks("causal", L))
+    assert_out(got, want, tol)
+    assert_cache(c.gpu, c.ref, S, start + S)
