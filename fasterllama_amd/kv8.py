@@ -195,8 +195,9 @@ class KV8Attention:
                 out_scale=None, seq_len_per_seq=None):
         """The prompt phase: q, k_new, v_new [B,S,H,D] at positions start_pos .. start_pos+S-1 (causal by the mask); returns
         out [B,H,S,D] float32.  seq_len_per_seq: int32 [B] on the device, the tokens that each sequence brings of them: the
-        padding behind is not stored, its output rows are zeros.  With cache.weights, the last weight_queries queries add theirs (0: all).  mask_tile_classes:
-        PrefillAttention.classify_mask of the whole [L, L] mask."""
+        padding behind is not stored, its output rows are zeros.  With cache.weights (up to size_per_head 128), the last weight_queries
+        queries add theirs (0: all); beyond that size, zero cache.weights and pass KV8Cache.of() the other arrays alone.
+        mask_tile_classes: PrefillAttention.classify_mask of the whole [L, L] mask."""
         B, H, L, D = self.shape
         S = q.shape[1] if q.dim() == 4 else 0
         _need(0 < S <= self.max_seq_len, f"q is [B, S, H, D] with 1 <= S <= max_seq_len = {self.max_seq_len}")

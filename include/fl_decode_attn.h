@@ -278,7 +278,9 @@ int fl_kv8_decode_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, c
  * attends to it, and its output rows are zeros; the next row of that sequence is start_pos + seq_len_per_seq[b].  An entry
  * outside [0, seq_len]: NaN output for that sequence, nothing stored.  (A padded prompt without it is stored whole, and its
  * padding cannot be overwritten row by row: see the order of appends above.)  With cache.weights, the last weight_queries
- * queries of every sequence add theirs (0 = all); served for size_per_head <= 128 (FL_ATTN_ERR_HEAD_DIM). */
+ * queries of every sequence add theirs (0 = all); served for size_per_head <= 128 (FL_ATTN_ERR_HEAD_DIM).  Beyond that size a
+ * prompt takes cache.weights = NULL.  It then leaves the array alone: where one is kept for the steps and evictions behind it,
+ * the caller zeroes the entries of the blocks that the prompt begins, since a step adds to them and an eviction compares them. */
 int fl_kv8_prefill_forward(const fl_attn_desc *desc, const fl_kv8_cache *cache, const fl_attn_io *io, int32_t seq_len,
                            const int32_t *seq_len_per_seq, int32_t weight_queries, void *hip_stream);
 

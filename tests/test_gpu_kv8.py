@@ -925,3 +925,31 @@ def test_wide_prompt_behind_a_long_context(gpu, D, T, start):
     got, want, tol = c.prompt(S, masks("causal", L))
     assert_out(got, want, tol)
     assert_cache(c.gpu, c.ref, S, start + S)
+
+
+@pytest.mark.parametrize("D,T", [(256, 64), (1024, 32)])
+def test_eviction_where_a_prompt_cannot_gather_weights(gpu, D, T):
+    """size_per_head beyond 128: the prompt goes through the same arrays without weights, whose entries the caller zeroes; the steps
+    behind it gather, and the eviction goes by them."""
+    import torch
+    from fasterllama_amd.kv8 import KV8Cache
+    L, S = 6 * T, 4 * T + 5
+    c = Case(gpu, 2, 2, D, L, T, "f16", 0, weights=True, max_seq_len=S)
+    raw, val, _ = c.feed(S, 3)
+    with pytest.raises(capi.FlAttnError):
+        c.op.prefill(*raw, c.gpu, c.table_d)
+    g = c.gpu
+    g.weights.zero_()
+    c.ref.weights[:] = 0
+    c.op.prefill(*raw, KV8Cache.of(T, g.k, g.v, g.k_scale, g.v_scale, g.k_tail, g.v_tail), c.table_d)
+    c.ref.step(*val, c.table, c.rows)
+    c.ref.weights[:] = 0
+    for step in range(3):
+        c.rows[:] = S + step
+        got, want, tol = c.decode(seed=50 + step)
+        assert_out(got, want, tol, f"step {step}")
+    assert_cache(c.gpu, c.ref, 3, S + 3)
+    c.ref.weights[:] = c.gpu.weights.cpu().numpy()  # (equal but for their last bits, by which close ones would differ)
+    kept, after = c.op.evict(c.gpu, 2, 1, S + 3)
+    want_kept, _ = kr.evict(c.ref, np.full(2, S + 3), 2, 1)
+    assert np.array_equal(kept.cpu().numpy(), want_kept) and (after.cpu().numpy() == 2 * T + 8).all()
