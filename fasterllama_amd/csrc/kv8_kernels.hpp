@@ -443,7 +443,7 @@ void kv8_attn_kernel(const Kv8Params p)
     constexpr int LPR = G::LPR, GPW = G::GPW, U = G::U, WT = G::WT, GR = G::GR;
     constexpr bool CHECK = WT > 32; // a trip may reach over the end of the rows (blocks are multiples of 32)
     static_assert(kKv8Waves * 64 == kCombineThreads, "the merge runs on a 256-thread workgroup");
-    __shared__ float s_o[kKv8Waves][D];
+    __shared__ __attribute__((aligned(16))) float s_o[kKv8Waves][D];
     __shared__ float s_m[kKv8Waves], s_l[kKv8Waves], s_t[kKv8Waves], s_red[kKv8Waves];
     __shared__ __attribute__((aligned(16))) char s_merge_bytes[PROMPT ? 16 : sizeof(MergeShared<D>)];
     constexpr int LDS_GRANULES = (int)sizeof(s_merge_bytes) / 8; // where one workgroup has all rows and does not merge
@@ -1209,11 +1209,12 @@ __device__ __forceinline__ int block_rank(bool flag, int *s_cnt, int &total)
 // weights move with it; in place, an entry moves to its own or a lower slot: NT entries are read before they are written.
 constexpr int kCountedBlocks = 64; // (each comes down to 16 reads of four keys)
 struct SelectShared {
-    uint32_t key[kCountedBlocks];
+    alignas(16) uint32_t key[kCountedBlocks]; // read four at a time
     int hist[256];
     int cnt[16];
     uint32_t pick[2]; // threshold byte, entries still wanted at it
 };
+static_assert(alignof(SelectShared) >= sizeof(uint4) && kCountedBlocks % 4 == 0, "the keys are read as uint4");
 template <int NT>
 __device__ __forceinline__ void select_blocks(const Kv8EvictParams &p, int bh, int rows, int *s_list, SelectShared &sh)
 {
