@@ -953,3 +953,64 @@ def test_eviction_where_a_prompt_cannot_gather_weights(gpu, D, T):
     kept, after = c.op.evict(c.gpu, 2, 1, S + 3)
     want_kept, _ = kr.evict(c.ref, np.full(2, S + 3), 2, 1)
     assert np.array_equal(kept.cpu().numpy(), want_kept) and (after.cpu().numpy() == 2 * T + 8).all()
+
+
+@pytest.mark.parametrize("D,T,rows", [(128, 64, 5000), (128, 32, 9000), (32, 128, 17000), (96, 32, 9001), (256, 64, 9000), (1024, 32, 2000)])
+@pytest.mark.parametrize("kind", [None, "even"])
+@pytest.mark.parametrize("ready", [True, False])
+def test_steps_of_many_splits(gpu, D, T, rows, kind, ready):
+    """More splits than a merge requests ahead, and more than a wave has lanes; `even`: -1e9 on every key, which then weigh the same."""
+    L = (rows // T + 2) * T
+    c = long_case(gpu, D, T, rows, L, nsplit=1024)
+    if not ready:  # the merge as a launch of its own
+        def without(call, *args):
+            c.op.io.flags = 0
+            capi.check(call(*args, 0))
+        c.op._enqueue = without
+    import torch
+    torch.cuda.synchronize()
+    before = c.ref.weights.copy()
+    m = np.full((1, L), -1e9, np.float32) if kind else None
+    raw, val, _ = c.feed(1, 3)
+    got = c.op.decode(*raw, c.gpu, c.table_d, start_pos=rows, attn_mask=c.t(m))
+    torch.cuda.synchronize()
+    want, tol = c.ref.step(*val, c.table, c.rows)
+    want, tol = want[:, :, 0], tol[..., 0]
+    if kind:
+        n = rows + 1
+        _, vv = c.ref.values(0, n)
+        want = vv.mean(1)[None]
+        tol = kr.U * (math.sqrt(n) + 64) * np.abs(vv).mean(1).max(-1)[None, :, None]
+        share = np.minimum(T, n - T * np.arange(-(-n // T))) / n
+        c.ref.weights[:, :, :share.size] = np.where(T * np.arange(share.size) >= rows, 0, before[:, :, :share.size]) + share
+    assert_out(got, want, tol)
+    assert_cache(c.gpu, c.ref)
+
+
+@pytest.mark.parametrize("D,T", [(64, 32), (128, 32), (512, 64)])
+def test_steps_that_fill_a_block_of_zeros(gpu, D, T):
+    c = Case(gpu, 1, 2, D, 3 * T, T, "f16", 0, weights=True)
+    for step in range(2 * T + 3):
+        c.rows[:] = step
+        raw, val, _ = c.feed(1, 100 + step)
+        q, k, v = (x.copy() for x in val)
+        if step < T:
+            k[:], v[:] = 0, 0
+        got = c.op.decode(c.t(q), c.t(k), c.t(v), c.gpu, c.table_d, start_pos=step)
+        want, tol = c.ref.step(q, k, v, c.table, c.rows)
+        assert_out(got, want[:, :, 0], tol[..., 0], f"step {step}")
+    assert_cache(c.gpu, c.ref, 2 * T + 3)
+    assert not c.gpu.k_scale[:, :, 0].cpu().numpy().any() and not c.gpu.k[:, :, :T].cpu().numpy().any()
+
+
+@pytest.mark.parametrize("D,T,start,S", [(128, 64, 0, 320), (64, 32, 77, 150), (128, 64, 1300, 40)])
+def test_block_weights_of_queries_that_weigh_their_keys_evenly(gpu, D, T, start, S):
+    L, W = -(-(start + S) // T) * T, 30
+    c = Case(gpu, 1, 2, D, L, T, "f16", start, weights=True, max_seq_len=S)
+    before, n = c.ref.weights.copy(), start + S
+    raw, val, _ = c.feed(S, 4)
+    c.op.prefill(*raw, c.gpu, c.table_d, start_pos=start, attn_mask=c.t(np.full((L, L), -1e9, np.float32)), weight_queries=W)
+    c.ref.step(*val, c.table, c.rows)
+    share = W * np.minimum(T, n - T * np.arange(-(-n // T))) / n
+    c.ref.weights[:, :, :share.size] = np.where(T * np.arange(share.size) >= start, 0, before[:, :, :share.size]) + share
+    assert_cache(c.gpu, c.ref, W, n)
