@@ -692,7 +692,8 @@ void kv8_attn_kernel(const Kv8Params p)
         }
     }
 
-    // The query as three digits per element.  A non-finite element makes the factor NaN, as it would every score.
+    // The query as three digits per element, to 2^-24 of the head's largest one: a score is off by that much of max|q| sum|k|, as
+    // sums in FP32 are.  A non-finite element makes the factor NaN, as it would every score.
     uint32_t qd[3][4];
     float qs;
     {

@@ -14,8 +14,8 @@
 //              element lies in [256, 512), a weight by 2^7: remainders stay clear of fp16's smallest steps;
 //   loads      a tile is half the bytes: one 16-byte chunk of K and of V per thread (D = 128), widened to fp16 on the way
 //              into LDS by all four waves together.
-// Bound by the matrix instructions and what stands between them: B=1, S=4096, 32 heads, causal: 289 us, 292 TFLOP executed (the
-// pairs counted twice) = 1.0 PFLOP/s, matrix pipe busy 53 % of the cycles; B=8, S=1024: 195 us, 0.75 PFLOP/s, of which 63 us
+// Bound by the matrix instructions and what stands between them: B=1, S=4096, 32 heads, causal: 288 us, 292 GFLOP executed (the
+// pairs counted twice) = 1.0 PFLOP/s, matrix pipe busy 53 % of the cycles; B=8, S=1024: 193 us, 0.75 PFLOP/s, of which 63 us
 // are what a workgroup does before and after its tiles.  Taken out one at a time (S=4096 / S=1024): the remainders' products
 // 219 / 163 us, the widening 272 / 196, the exponentials 268 / 194, reading and rotating the queries 265 / 168.
 #pragma once
@@ -580,9 +580,9 @@ __global__ __launch_bounds__(256) void kv8_prompt_merge_kernel(const Kv8PromptPa
 // much traffic at the L1 as the products take.  With NQ = 2 or 4 a workgroup is done sooner, where there are few of them.  The
 // blocks that the mask leaves something of are listed first, with their classes, as in the attention kernel.
 // grid = B*H * ceil(keys of the longest sequence / (256 / NQ)), heads fastest: under a causal mask the first keys' workgroups are
-// the longest and start first, and an XCD keeps to its heads' operands; block = 256.  32 heads, 4096 queries, causal, all counted:
-// 160 us (107 for the products at the library's rate; key groups fastest, unstaged, classes behind each other 277).  Sums are formed
-// in one order, so they are the same from run to run.
+// the longest and start first, and an XCD keeps to its heads' operands; block = 256.  32 heads, 4096 queries, causal, all counted
+// (two streams): 195-208 us (107 for the products at the library's rate; key groups fastest, classes behind each other 277).  Sums
+// are formed in one order, so they are the same from run to run.
 constexpr int kQueryListCap = 1024; // 32-query blocks per pass
 template <int D, bool STAGED>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 8)))
