@@ -29,7 +29,9 @@ namespace flattn {
 // Weights times V scale enter the second product relative to a query's largest such product, times 2^7; kLazyMax = 8 more stay below
 // 65504.  The remainder's smallest step is 2^-24: a weight is held to 2^-22 of itself or to 2^-32 of that largest product.
 constexpr float kKv8WeightExp = 7.0f;
-constexpr int kKv8LeastScaleExp = -40; // a block's scale is 0 or at least 2^-31 (fp16's smallest step over 127): 0 counts as 2^-40
+// A block's scale is 0 or lies in [2^-31, 2^10) (fp16's steps over 127).  Zeros count as 2^-80: small enough to leave the reference to the
+// others where they take e^-50 of the weight, while the sum of the weights, in units of the reference's score, stays below 2^127.
+constexpr int kKv8LeastScaleExp = -80;
 
 struct Kv8PromptParams {
     Kv8Params k;
@@ -439,7 +441,7 @@ void kv8_prefill_attn_kernel(const Kv8PromptParams pp)
                 const float mx = cross_half_max(max16(st)) * cs;
                 const float over = (mx - m) + (vexp - r) + vfrac; // of this tile's largest product over the reference (-inf: all masked)
                 if (__ballot(over > kLazyMax) != 0ull) { // wave-uniform
-                    const float m_new = over > 0.f ? mx : m, r_new = over > 0.f ? vexp : r; // (what l counts stays within 2^57 of 1)
+                    const float m_new = over > 0.f ? mx : m, r_new = over > 0.f ? vexp : r; // (a weight that l counts stays below 2^98)
                     const float alpha = __builtin_amdgcn_exp2f((m - m_new) + (r - r_new));
                     l *= __builtin_amdgcn_exp2f(m - m_new);
                     m = m_new;

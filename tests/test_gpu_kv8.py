@@ -1014,3 +1014,21 @@ def test_block_weights_of_queries_that_weigh_their_keys_evenly(gpu, D, T, start,
     share = W * np.minimum(T, n - T * np.arange(-(-n // T))) / n
     c.ref.weights[:, :, :share.size] = np.where(T * np.arange(share.size) >= start, 0, before[:, :, :share.size]) + share
     assert_cache(c.gpu, c.ref, W, n)
+
+
+@pytest.mark.parametrize("bias", [10.0, 30.0, 50.0])
+@pytest.mark.parametrize("D,T,S", [(128, 64, 320), (128, 128, 156), (32, 32, 75), (64, 64, 1100), (256, 64, 100)])
+def test_zeros_that_take_the_weight(gpu, D, T, S, bias):
+    """A block of zeros with scores `bias` higher: next to nothing is left for the others, and all of the output comes from it."""
+    L = -(-S // T) * T
+    c = Case(gpu, 1, 2, D, L, T, "f32", 0, max_seq_len=S, weights=D <= 128)
+    _, val, _ = c.feed(S, 3)
+    q, k, v = (x.copy() for x in val)
+    v[:, :T] = 0
+    m = np.full((1, L), -bias, np.float32)
+    m[:, :T] = 0
+    m = np.broadcast_to(m, (L, L))
+    got, want, tol = prompt_of(c, q, k, v, m)
+    # beside the products' errors, a score rounds next to a mask entry of `bias`, before and after the change of base: 4 U of it
+    assert_out(got, want, tol * (1 + 4 * bias / 64), f"bias {bias}")
+    assert_cache(c.gpu, c.ref, S, S)
